@@ -40,12 +40,13 @@ typedef enum sdmi_status {
 typedef enum sdmi_dtype {
     SDMI_DTYPE_BF16 = 0, SDMI_DTYPE_F16 = 1,
     SDMI_DTYPE_F32_PLANES = 2,   /* sdmi_pack_* only: the six bf16 piece planes of the fp32 mode (see sdmi_f32_split3) */
-    SDMI_DTYPE_F16_TO_BF16 = 3   /* sdmi_groupnorm / sdmi_groupnorm_noalloc / sdmi_layernorm only: input f16 (the residual
+    SDMI_DTYPE_F16_TO_BF16 = 3,  /* sdmi_groupnorm / sdmi_groupnorm_noalloc / sdmi_layernorm only: input f16 (the residual
                                     stream of the bf16 operand policy), output bf16 (an MFMA operand) */
+    SDMI_DTYPE_F32 = 4           /* the block-scaled operators only (sdmi_mx_*, sdmi_rmsnorm, sdmi_gated) */
 } sdmi_dtype;
 
 const char* sdmi_status_str(int status);
-int sdmi_abi_version(void);   /* 13: + sdmi_gemm_args.tile_n == 64 (the 64-column tile, tile_m 64 | 128), ln_stats_slots up to 48; 12: + sdmi_gemm_args.ln_colsum / ln_stats / row_stats_out (LayerNorm folded into the projection, row statistics travelling with the residual stream), sdmi_gemm_row_stats_slots, sdmi_row_stats, sdmi_xattn_block (the cross-attention half of a transformer block as one launch); 11: + sdmi_gemm_args.out_f16 / res_f16 / a_f16 / dup_rows, SDMI_DTYPE_F16_TO_BF16, sdmi_probe_mfma, sdmi_probe_copy (measurement aids); 10: + sdmi_gemm_args.tile_n == 256, sdmi_gemm_wide_applies; 9: + sdmi_f32_attention_vae, sdmi_f32_nchw_to_nhwc takes a scale; 8: + sdmi_gemm_args.ln_gamma/ln_beta/ln_eps, sdmi_gemm_panel_applies; 7: + sdmi_gemm_args.algo; 6: + sdmi_attention_vae; 5: + sdmi_pack_*; 4: + sdmi_groupnorm_noalloc, SDMI_ERR_TOO_LARGE (3: + sdmi_f32_embed_tokens,
+int sdmi_abi_version(void);   /* 14: + the block-scaled operators (sdmi_mx_*, sdmi_rmsnorm, sdmi_gated), SDMI_DTYPE_F32; 13: + sdmi_gemm_args.tile_n == 64 (the 64-column tile, tile_m 64 | 128), ln_stats_slots up to 48; 12: + sdmi_gemm_args.ln_colsum / ln_stats / row_stats_out (LayerNorm folded into the projection, row statistics travelling with the residual stream), sdmi_gemm_row_stats_slots, sdmi_row_stats, sdmi_xattn_block (the cross-attention half of a transformer block as one launch); 11: + sdmi_gemm_args.out_f16 / res_f16 / a_f16 / dup_rows, SDMI_DTYPE_F16_TO_BF16, sdmi_probe_mfma, sdmi_probe_copy (measurement aids); 10: + sdmi_gemm_args.tile_n == 256, sdmi_gemm_wide_applies; 9: + sdmi_f32_attention_vae, sdmi_f32_nchw_to_nhwc takes a scale; 8: + sdmi_gemm_args.ln_gamma/ln_beta/ln_eps, sdmi_gemm_panel_applies; 7: + sdmi_gemm_args.algo; 6: + sdmi_attention_vae; 5: + sdmi_pack_*; 4: + sdmi_groupnorm_noalloc, SDMI_ERR_TOO_LARGE (3: + sdmi_f32_embed_tokens,
                                  sdmi_f32_attention_d64_causal, sdmi_gemm_args.act == 2; 2: dtype, fp32 mode) */
 
 /* ------------------------------------------------------------------------------------------
@@ -409,6 +410,75 @@ int sdmi_diag_gaussian(const float* parameters, float* mean, float* log_var, flo
 int sdmi_mul_add(const float* a, const float* b, const float* c, float* out, int64_t n, void* stream);
 
 int sdmi_image_to_u8(const float* x, uint8_t* out, int32_t nb, int32_t C, int64_t hw, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Block-scaled (MX) operators: a product with 4-bit weights and 8- or 4-bit activations, and what feeds it.  They stand
+ * beside sdmi_gemm, sdmi_layernorm and the GEGLU epilogue for models that are served below 16 bits (feed-forwards and
+ * projections of language models and of the text towers in front of a UNet).
+ *
+ * Format (OCP Microscaling v1.0): blocks of 32 consecutive values of a row share a scale 2^(byte - 127); elements are e4m3
+ * (SDMI_MX_FP8, largest 448) or e2m1 (SDMI_MX_FP4, largest 6).  byte = max(0, floor(log2 max|x|) - emax + 127) with emax 8
+ * or 2; an element is x / scale rounded to nearest even and saturated.  A block that holds a NaN or an infinity becomes
+ * NaN as a whole (byte 255).  K is any positive number up to 2^24; the last block is filled with zeros.
+ *   activations: codes [rows][Kp bytes] (FP8) or [rows][Kp / 2 bytes] (FP4, even k in the low nibble), Kp = K rounded up
+ *       to 128; scales [Kp / 128][rows][4 bytes] (the four blocks of a row's 128 values).  Sizes: sdmi_mx_codes_bytes,
+ *       sdmi_mx_scales_bytes (-1 for sizes that are refused).
+ *   weights: an opaque order of the same values (sdmi_mx_pack_linear).
+ * dtype / out_dtype: SDMI_DTYPE_BF16 | _F16 | _F32.  Leading dimensions count elements; rows may be strided, the inner
+ * stride is 1.  16-byte aligned rows (pointer, and leading dimension a multiple of 8, or 4 for fp32) are read in vectors,
+ * others element by element.  Codes, scales, packed weights, gamma and workspaces are 16-byte aligned (else SDMI_ERR_ALIGNMENT).
+ * rows == 0 is a valid empty call.  Outputs may not overlap inputs.
+ *   sdmi_mx_quantize:   [rows, K] -> codes, scales
+ *   sdmi_mx_dequantize: the values that codes and scales stand for (bf16 and fp32 hold them exactly, but for bf16's range)
+ *   sdmi_rmsnorm:       s = x + res (res NULL: s = x), y = s / sqrt(mean(s^2) + eps) * gamma; s in fp32, stored in x's type
+ *       to sum_out [rows, C] (required with res, ignored without).  C <= SDMI_RMSNORM_MAX_C.  fmt SDMI_MX_NONE: out is
+ *       [rows, C] of out_dtype; else out holds codes, and scales the scales.
+ *   sdmi_gated:         y = a * act(b), x = [a | b] with halves of `inner` columns (the order of the GEGLU projection,
+ *       ldm/modules/attention.py:89); act 0 GELU (erf), 1 SiLU; fmt, out, scales as above.
+ * ---------------------------------------------------------------------------------------- */
+#define SDMI_MX_NONE 0
+#define SDMI_MX_FP8 1
+#define SDMI_MX_FP4 2
+#define SDMI_RMSNORM_MAX_C 16384
+int64_t sdmi_mx_codes_bytes(int64_t rows, int64_t K, int32_t fmt);
+int64_t sdmi_mx_scales_bytes(int64_t rows, int64_t K);
+int sdmi_mx_quantize(const void* x, int64_t ldx, int64_t rows, int64_t K, int32_t dtype, void* codes, void* scales,
+                     int32_t fmt, void* stream);
+int sdmi_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t K, int32_t fmt, void* out,
+                       int64_t ld_out, int32_t out_dtype, void* stream);
+int sdmi_rmsnorm(const void* x, int64_t ldx, const void* res, int64_t ld_res, const float* gamma, float eps, int64_t rows,
+                 int64_t C, int32_t dtype, void* sum_out, void* out, int32_t out_dtype, void* scales, int32_t fmt,
+                 void* stream);
+int sdmi_gated(const void* x, int64_t ldx, int64_t rows, int64_t inner, int32_t dtype, int32_t act, void* out,
+               int32_t out_dtype, void* scales, int32_t fmt, void* stream);
+
+/* w [N, K] -> 4-bit codes and scales in the order of the product, padded to whole groups of 64 rows and 128 columns. */
+int64_t sdmi_mx_weight_codes_bytes(int64_t N, int64_t K);
+int64_t sdmi_mx_weight_scales_bytes(int64_t N, int64_t K);
+int sdmi_mx_pack_linear(const void* w, int64_t ldw, int64_t N, int64_t K, int32_t dtype, void* codes, void* scales,
+                        void* stream);
+
+/* out[m, n] = sum_k x[m, k] w[n, k] + bias[n] + res[m, n]: block-scaled operands, fp32 accumulation in an order that
+ * depends on the sizes alone, one rounding to out_dtype. */
+typedef struct sdmi_mx_gemm_args {
+    const void* x;           /* [M, K] of x_dtype, quantised to fmt on the way, or NULL: x_codes / x_scales hold it */
+    const void* x_codes;
+    const void* x_scales;
+    const void* w_codes;
+    const void* w_scales;
+    const float* bias;       /* [N] or NULL */
+    const void* res;         /* [M, N] of out_dtype or NULL */
+    void* out;               /* [M, N] of out_dtype */
+    void* workspace;         /* sdmi_mx_gemm_workspace_bytes(args) bytes; NULL where that is 0 */
+    int64_t workspace_bytes;
+    int64_t M, N, K;
+    int64_t ldx, ld_res, ld_out;
+    int32_t x_dtype, out_dtype;
+    int32_t fmt;             /* of the activations */
+    int32_t reserved;        /* 0 */
+} sdmi_mx_gemm_args;
+int64_t sdmi_mx_gemm_workspace_bytes(const sdmi_mx_gemm_args* args);   /* -1: sizes that sdmi_mx_gemm refuses */
+int sdmi_mx_gemm(const sdmi_mx_gemm_args* args, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Measurement aids (no counterpart in the reference; they compute nothing the path uses).  bench.py times them with

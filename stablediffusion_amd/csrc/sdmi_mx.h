@@ -1,0 +1,140 @@
+// Block-scaled (MX) operands: element formats, layouts and the block quantiser shared by the sdmi_mx kernels.
+//
+// A block is 32 consecutive values of a row with one power-of-two scale, held as its exponent + 127 in a byte (255: the
+// block is NaN).  Elements are e4m3 (MX8) or e2m1 (MX4).  K is padded to whole k-steps of 128 = 4 blocks - the depth of
+// v_mfma_scale_f32_16x16x128_f8f6f4 - with zero codes and scale bytes 0.
+//   activations: codes [rows][Kp] bytes (MX8) or [rows][Kp / 2] (MX4, even k in the low nibble);
+//                scales [Kp / 128][rows][4]: the four bytes of one row and k-step are one dword, and the rows of a tile are
+//                contiguous, so that a tile's scales move as whole lines
+//   weights:     in the order the matrix instruction reads them, see sdmi_mx_gemm.hip
+#pragma once
+#include "sdmi_common.h"
+
+constexpr int MX_BLOCK = 32, MX_KSTEP = 128;
+
+__host__ __device__ __forceinline__ int64_t mx_ksteps(int64_t K) { return (K + MX_KSTEP - 1) / MX_KSTEP; }
+__host__ __device__ __forceinline__ int64_t mx_row_bytes(int64_t K, int fmt) { return mx_ksteps(K) * (fmt == SDMI_MX_FP8 ? 128 : 64); }
+
+// Source types of the element-wise kernels: 0 bf16, 1 f16, 2 fp32 (sdmi_dtype mapped by mx_src_type on the host).
+static inline int mx_src_type(int32_t dtype) {
+    return dtype == SDMI_DTYPE_BF16 ? 0 : dtype == SDMI_DTYPE_F16 ? 1 : dtype == SDMI_DTYPE_F32 ? 2 : -1;
+}
+template <int T> struct MxElem { typedef unsigned short type; };
+template <> struct MxElem<2> { typedef float type; };
+
+template <int T> __device__ __forceinline__ float mx_to_f32(typename MxElem<T>::type v) {
+    if constexpr (T == 2) return v;
+    else return elem_to_f32<T>(v);
+}
+
+// 8 consecutive values from p[0..]; `n` of them exist (the others read as 0).  vec: p is aligned to a 16-byte vector.
+template <int T> __device__ __forceinline__ void mx_load8(const typename MxElem<T>::type* p, int n, bool vec, float* f) {
+    if (vec && n >= 8) {
+        if constexpr (T == 2) {
+            const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { f[j] = a[j]; f[4 + j] = b[j]; }
+        } else {
+            elem_unpack8<T>(*reinterpret_cast<const uint4*>(p), f);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = j < n ? mx_to_f32<T>(p[j]) : 0.0f;
+    }
+}
+// 8 consecutive values to p[0..], of which `n` exist.
+template <int T> __device__ __forceinline__ void mx_store8(typename MxElem<T>::type* p, int n, bool vec, const float* f) {
+    if (vec && n >= 8) {
+        if constexpr (T == 2) {
+            reinterpret_cast<f32x4*>(p)[0] = (f32x4){f[0], f[1], f[2], f[3]};
+            reinterpret_cast<f32x4*>(p)[1] = (f32x4){f[4], f[5], f[6], f[7]};
+        } else {
+            *reinterpret_cast<uint4*>(p) = elem_pack8<T>(f);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (j < n) {
+                if constexpr (T == 2) p[j] = f[j];
+                else p[j] = elem_from_f32<T>(f[j]);
+            }
+        }
+    }
+}
+
+// Lane exchanges inside a row of 16 lanes, without LDS.
+template <int CTRL> __device__ __forceinline__ unsigned mx_dpp(unsigned v) {
+    return (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
+}
+
+// The shared exponent of a block from the bits of its largest magnitude: floor(log2 max) is the exponent field (0 for
+// subnormals, whose byte is 0 in any case), the scale lies FMT's largest exponent below it.  255 marks NaN and infinity:
+// their bits are the largest, so the integer maximum finds them.
+template <int FMT> __device__ __forceinline__ unsigned mx_scale_byte(unsigned amax_bits) {
+    const unsigned e = amax_bits >> 23, emax = FMT == SDMI_MX_FP8 ? 8u : 2u;
+    return e == 255u ? 255u : (e > emax ? e - emax : 0u);
+}
+// The reciprocal of the scale: 2^(127 - byte), exact and normal for every byte <= 252, so that x * it is x / scale.
+__device__ __forceinline__ float mx_inv_scale(unsigned byte) { return __uint_as_float((254u - byte) << 23); }
+
+// 8 scaled values -> codes: 8 bytes (MX8) or 4 bytes (MX4, in .x).  Round to nearest even, saturating: the 8-bit convert
+// would turn what rounds past 448 into NaN, so it is clamped first; the 4-bit one saturates by itself.
+template <int FMT> __device__ __forceinline__ uint2 mx_codes8(const float* f, float inv) {
+    uint2 r = {0u, 0u};
+    if constexpr (FMT == SDMI_MX_FP8) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __builtin_amdgcn_fmed3f(f[j] * inv, -448.0f, 448.0f);
+        int a = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+        a = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], a, true);
+        int b = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
+        b = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], b, true);
+        r.x = (unsigned)a;
+        r.y = (unsigned)b;
+    } else {
+        unsigned a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, f[0] * inv, f[1] * inv, 1.0f, 0);
+        a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, f[2] * inv, f[3] * inv, 1.0f, 1);
+        a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, f[4] * inv, f[5] * inv, 1.0f, 2);
+        a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, f[6] * inv, f[7] * inv, 1.0f, 3);
+        r.x = a;
+    }
+    return r;
+}
+
+__device__ __forceinline__ unsigned mx_amax8(const float* f) {
+    unsigned m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(f[j]) & 0x7fffffffu);
+    return m;
+}
+
+// One k-step of one row, held by 16 consecutive lanes with 8 values each (4 lanes a block): `codes` gets this lane's codes,
+// the return value is the row's scale dword (the same in the 16 lanes).  All 16 lanes have to take part.
+template <int FMT> __device__ __forceinline__ unsigned mx_quantise8(const float* f, int lane, uint2& codes) {
+    unsigned m = mx_amax8(f);
+    m = max(m, mx_dpp<0xB1>(m));                          // quad_perm 1 0 3 2
+    m = max(m, mx_dpp<0x4E>(m));                          // quad_perm 2 3 0 1
+    const unsigned byte = mx_scale_byte<FMT>(m);
+    codes = mx_codes8<FMT>(f, mx_inv_scale(min(byte, 252u)));
+    if (byte == 255u) codes = (uint2){0u, 0u};            // the scale alone says NaN
+    unsigned dw = byte << (8 * ((lane & 15) >> 2));
+    dw |= mx_dpp<0x124>(dw);                              // row_ror 4
+    dw |= mx_dpp<0x128>(dw);                              // row_ror 8
+    return dw;
+}
+
+// GELU by the error function, x Phi(x), for any magnitude: Phi(-|x|) = erfc(z) / 2 with z = |x| / sqrt 2, and
+// erfc(z) = exp(-z^2) t P(t), t = 1 / (1 + 0.375 z), P a degree-6 polynomial fitted to exp(z^2) erfc(z) on [0, 10]
+// (relative error 6.4e-7).  Written from the small side, so that the tail of negative x keeps its relative precision.
+__device__ __forceinline__ float mx_gelu(float x) {
+    const float z = fabsf(x) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.375f, z, 1.0f));
+    float p = fmaf(-1.350968426e-01f, t, 3.879412549e-01f);
+    p = fmaf(p, t, -1.296022628e-01f);
+    p = fmaf(p, t, 2.830651671e-01f);
+    p = fmaf(p, t, 1.666631723e-01f);
+    p = fmaf(p, t, 2.156894433e-01f);
+    p = fmaf(p, t, 2.113394301e-01f);
+    const float half = 0.5f * p * t * __expf(-0.5f * x * x);     // Phi(-|x|); z^2 as x^2 / 2: one rounding before the exponential
+    return x * (x < 0.0f ? half : 1.0f - half);
+}

@@ -1,0 +1,330 @@
+// sdmi_mx: the element-wise and row-wise operators around the block-scaled product (sdmi_mx_gemm.hip): quantisation of a
+// matrix and its reading back, the gated activation, the RMS norm with the residual's addition - each with a 16-bit, fp32 or
+// block-scaled result - and the packing of weights.  All of them are bound by bytes: every input is read once in 16-byte
+// vectors, statistics stay in registers, the result is written once in the form its reader takes.
+#include "sdmi_mx.h"
+
+// ---- one k-step per 16 lanes -------------------------------------------------------------------------------------------
+// A block of 256 threads owns a tile of 16 rows x 4 k-steps (512 values): 16 lanes hold one k-step of one row, 8 values a
+// lane, and walk the four k-steps.  So a row's 1 KB is read in 256-byte runs, and the 16 scale dwords of a k-step lie next
+// to each other.
+constexpr int EL_ROWS = 16, EL_STEPS = 4;
+
+struct MxElemArgs {
+    const void* x;
+    int64_t ldx, rows, K;      // gated: K = the width of one half, the gate starts at column K
+    void* out;                 // FMT none: [rows][ld_out] of the source's type or the given one
+    int64_t ld_out;
+    unsigned char* codes;
+    unsigned char* scales;
+    unsigned ktiles;
+    int vec_in, vec_gate, vec_out;
+};
+
+// OP 0: x   1: a gelu(b)   2: a silu(b)        FMT -1: plain result of type TO
+template <int T, int OP, int FMT, int TO>
+__global__ __launch_bounds__(256) void sdmi_mx_elem_kernel(MxElemArgs p) {
+    typedef typename MxElem<T>::type E;
+    const unsigned tile_r = blockIdx.x / p.ktiles, tile_k = blockIdx.x - tile_r * p.ktiles;
+    const int lane = threadIdx.x & 63, sub = threadIdx.x & 15;
+    const int64_t row = (int64_t)tile_r * EL_ROWS + (threadIdx.x >> 4);
+    const int64_t nsteps = mx_ksteps(p.K);
+    const int64_t src_row = row < p.rows ? row : p.rows - 1;     // (the 16 lanes of a row past the end work on the last one and store nothing)
+    const E* const xr = reinterpret_cast<const E*>(p.x) + src_row * p.ldx;
+    float f[EL_STEPS][8], g[OP ? EL_STEPS : 1][8];
+#pragma unroll
+    for (int s = 0; s < EL_STEPS; ++s) {
+        const int64_t k0 = ((int64_t)tile_k * EL_STEPS + s) * MX_KSTEP + sub * 8;
+        const int n = (int)max((int64_t)0, min((int64_t)8, p.K - k0));
+        mx_load8<T>(xr + k0, n, p.vec_in, f[s]);
+        if constexpr (OP != 0) mx_load8<T>(xr + p.K + k0, n, p.vec_gate, g[s]);
+    }
+#pragma unroll
+    for (int s = 0; s < EL_STEPS; ++s) {
+        const int64_t step = (int64_t)tile_k * EL_STEPS + s;
+        if (step >= nsteps) break;                               // (uniform)
+        const int64_t k0 = step * MX_KSTEP + sub * 8;
+        const int n = (int)max((int64_t)0, min((int64_t)8, p.K - k0));
+        if constexpr (OP == 1) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[s][j] *= mx_gelu(g[s][j]);
+        } else if constexpr (OP == 2) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[s][j] *= silu_f(g[s][j]);
+        }
+        if constexpr (FMT < 0) {
+            if (row < p.rows && n > 0)
+                mx_store8<TO>(reinterpret_cast<typename MxElem<TO>::type*>(p.out) + row * p.ld_out + k0, n, p.vec_out, f[s]);
+        } else {
+            uint2 c;
+            const unsigned dw = mx_quantise8<FMT>(f[s], lane, c);
+            if (row < p.rows) {
+                if constexpr (FMT == SDMI_MX_FP8)
+                    *reinterpret_cast<uint2*>(p.codes + row * nsteps * 128 + k0) = c;
+                else
+                    *reinterpret_cast<unsigned*>(p.codes + row * nsteps * 64 + (k0 >> 1)) = c.x;
+                if (sub == 0) *reinterpret_cast<unsigned*>(p.scales + (step * p.rows + row) * 4) = dw;
+            }
+        }
+    }
+}
+
+// The values that codes and scales stand for.  Every code has at most four significant bits: a bf16 holds the value exactly
+// (down to its subnormals), an f16 rounds it to its own range.
+template <int FMT, int TO>
+__global__ __launch_bounds__(256) void sdmi_mx_dequantise_kernel(MxElemArgs p) {
+    const unsigned tile_r = blockIdx.x / p.ktiles, tile_k = blockIdx.x - tile_r * p.ktiles;
+    const int sub = threadIdx.x & 15;
+    const int64_t row = (int64_t)tile_r * EL_ROWS + (threadIdx.x >> 4), nsteps = mx_ksteps(p.K);
+    if (row >= p.rows) return;
+    uint2 c[EL_STEPS];
+    unsigned char sc[EL_STEPS];
+#pragma unroll
+    for (int s = 0; s < EL_STEPS; ++s) {
+        const int64_t step = (int64_t)tile_k * EL_STEPS + s;
+        if (step >= nsteps) break;
+        if constexpr (FMT == SDMI_MX_FP8) c[s] = *reinterpret_cast<const uint2*>(p.codes + row * nsteps * 128 + step * 128 + sub * 8);
+        else c[s].x = *reinterpret_cast<const unsigned*>(p.codes + row * nsteps * 64 + step * 64 + sub * 4);
+        sc[s] = p.scales[(step * p.rows + row) * 4 + (sub >> 2)];
+    }
+#pragma unroll
+    for (int s = 0; s < EL_STEPS; ++s) {
+        const int64_t step = (int64_t)tile_k * EL_STEPS + s;
+        if (step >= nsteps) break;
+        const int64_t k0 = step * MX_KSTEP + sub * 8;
+        const int n = (int)max((int64_t)0, min((int64_t)8, p.K - k0));
+        if (n == 0) continue;
+        float f[8];
+        if constexpr (FMT == SDMI_MX_FP8) {
+            const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[s].x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[s].x, true);
+            const f32x2 d = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[s].y, false), e = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[s].y, true);
+            f[0] = a[0]; f[1] = a[1]; f[2] = b[0]; f[3] = b[1]; f[4] = d[0]; f[5] = d[1]; f[6] = e[0]; f[7] = e[1];
+        } else {
+            const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[s].x, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[s].x, 1.0f, 1);
+            const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[s].x, 1.0f, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[s].x, 1.0f, 3);
+            f[0] = a[0]; f[1] = a[1]; f[2] = b[0]; f[3] = b[1]; f[4] = d[0]; f[5] = d[1]; f[6] = e[0]; f[7] = e[1];
+        }
+        // 2^(byte - 127): byte 0 is the subnormal 2^-127, byte 255 a NaN
+        const unsigned byte = sc[s];
+        const float scale = __uint_as_float(byte == 0u ? 0x00400000u : byte == 255u ? 0x7fc00000u : byte << 23);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] *= scale;
+        mx_store8<TO>(reinterpret_cast<typename MxElem<TO>::type*>(p.out) + row * p.ld_out + k0, n, p.vec_out, f);
+    }
+}
+
+// ---- RMS norm ----------------------------------------------------------------------------------------------------------
+// s = x + res (stored in x's type), y = s / sqrt(mean s^2 + eps) * gamma, of the fp32 sum.  TPR threads hold a row in
+// registers, U chunks of 8 values each, so that a row is read once; the sum of squares is an fp32 tree over those threads.
+struct MxNormArgs {
+    const void* x;
+    const void* res;           // NULL: s = x
+    const float* gamma;
+    void* sum_out;
+    void* out;
+    unsigned char* codes;
+    unsigned char* scales;
+    int64_t ldx, ld_res, rows, C;
+    float eps;
+    int vec_x, vec_res, vec_out;
+};
+
+template <int T, int FMT, int TO, int TPR, int U>
+__global__ __launch_bounds__(256) void sdmi_rmsnorm_kernel(MxNormArgs p) {
+    typedef typename MxElem<T>::type E;
+    constexpr int RPB = 256 / TPR;
+    __shared__ float part[RPB][TPR / 64];
+    const int t = threadIdx.x % TPR, r = threadIdx.x / TPR, lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * RPB + r, srow = row < p.rows ? row : p.rows - 1;
+    const E* const xr = reinterpret_cast<const E*>(p.x) + srow * p.ldx;
+    float f[U][8], q[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t c0 = ((int64_t)u * TPR + t) * 8;
+        const int n = (int)max((int64_t)0, min((int64_t)8, p.C - c0));
+        mx_load8<T>(xr + c0, n, p.vec_x, f[u]);
+    }
+    if (p.res) {
+        const E* const rr = reinterpret_cast<const E*>(p.res) + srow * p.ld_res;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t c0 = ((int64_t)u * TPR + t) * 8;
+            const int n = (int)max((int64_t)0, min((int64_t)8, p.C - c0));
+            mx_load8<T>(rr + c0, n, p.vec_res, q[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[u][j] += q[u][j];
+    }
+    float ss = 0.0f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = fmaf(f[u][j], f[u][j], ss);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
+    if constexpr (TPR > 64) {
+        if (lane == 0) part[r][t >> 6] = ss;
+        __syncthreads();
+        ss = 0.0f;
+#pragma unroll
+        for (int w = 0; w < TPR / 64; ++w) ss += part[r][w];
+    }
+    const float rstd = 1.0f / sqrtf(ss / (float)p.C + p.eps);
+    const int64_t nsteps = mx_ksteps(p.C);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t c0 = ((int64_t)u * TPR + t) * 8;
+        const int n = (int)max((int64_t)0, min((int64_t)8, p.C - c0));
+        if (p.sum_out && row < p.rows && n > 0)
+            mx_store8<T>(reinterpret_cast<E*>(p.sum_out) + row * p.C + c0, n, p.vec_out, f[u]);
+        float gm[8];
+        mx_load8<2>(p.gamma + c0, n, true, gm);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) gm[j] *= f[u][j] * rstd;
+        if constexpr (FMT < 0) {
+            if (row < p.rows && n > 0)
+                mx_store8<TO>(reinterpret_cast<typename MxElem<TO>::type*>(p.out) + row * p.C + c0, n, p.vec_out, gm);
+        } else {
+            const int64_t step = c0 / MX_KSTEP;
+            if (step >= nsteps) continue;                        // (whole groups of 16 lanes)
+            uint2 c;
+            const unsigned dw = mx_quantise8<FMT>(gm, lane, c);
+            if (row < p.rows) {
+                if constexpr (FMT == SDMI_MX_FP8)
+                    *reinterpret_cast<uint2*>(p.codes + row * nsteps * 128 + c0) = c;
+                else
+                    *reinterpret_cast<unsigned*>(p.codes + row * nsteps * 64 + (c0 >> 1)) = c.x;
+                if ((lane & 15) == 0) *reinterpret_cast<unsigned*>(p.scales + (step * p.rows + row) * 4) = dw;
+            }
+        }
+    }
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------------------
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static bool vec_rows(const void* p, int64_t ld, int type) { return aligned16(p) && ld % (type == 2 ? 4 : 8) == 0; }
+static bool fmt_ok(int32_t fmt) { return fmt == SDMI_MX_FP8 || fmt == SDMI_MX_FP4; }
+constexpr int64_t MX_MAX_K = (int64_t)1 << 24, MX_MAX_ROWS = ((int64_t)1 << 31) - 1;
+
+extern "C" int64_t sdmi_mx_codes_bytes(int64_t rows, int64_t K, int32_t fmt) {
+    return rows < 0 || K <= 0 || !fmt_ok(fmt) ? -1 : rows * mx_row_bytes(K, fmt);
+}
+extern "C" int64_t sdmi_mx_scales_bytes(int64_t rows, int64_t K) { return rows < 0 || K <= 0 ? -1 : rows * mx_ksteps(K) * 4; }
+
+// Whether the tiles of a launch fit a grid (grid.x < 2^31); `ktiles` is set.
+static bool elem_grid(int64_t rows, int64_t K, unsigned* ktiles, unsigned* blocks) {
+    const int64_t kt = (mx_ksteps(K) + EL_STEPS - 1) / EL_STEPS, n = (rows + EL_ROWS - 1) / EL_ROWS * kt;
+    *ktiles = (unsigned)kt;
+    *blocks = (unsigned)n;
+    return n < ((int64_t)1 << 31);
+}
+
+template <int T, int OP>
+static int elem_launch(const MxElemArgs& a, int fmt, int to, unsigned blocks, hipStream_t st) {
+    if (fmt == SDMI_MX_FP8) sdmi_mx_elem_kernel<T, OP, SDMI_MX_FP8, 0><<<blocks, 256, 0, st>>>(a);
+    else if (fmt == SDMI_MX_FP4) sdmi_mx_elem_kernel<T, OP, SDMI_MX_FP4, 0><<<blocks, 256, 0, st>>>(a);
+    else if constexpr (OP == 0) return SDMI_ERR_BAD_ARG;
+    else if (to == 0) sdmi_mx_elem_kernel<T, OP, -1, 0><<<blocks, 256, 0, st>>>(a);
+    else if (to == 1) sdmi_mx_elem_kernel<T, OP, -1, 1><<<blocks, 256, 0, st>>>(a);
+    else sdmi_mx_elem_kernel<T, OP, -1, 2><<<blocks, 256, 0, st>>>(a);
+    SDMI_CHECK_LAUNCH();
+    return SDMI_OK;
+}
+
+extern "C" int sdmi_mx_quantize(const void* x, int64_t ldx, int64_t rows, int64_t K, int32_t dtype, void* codes, void* scales,
+                                int32_t fmt, void* stream) {
+    const int t = mx_src_type(dtype);
+    if (!x || !codes || !scales || t < 0 || !fmt_ok(fmt) || rows < 0 || K <= 0 || K > MX_MAX_K || ldx < K || rows > MX_MAX_ROWS) return SDMI_ERR_BAD_ARG;
+    if (!aligned16(codes) || !aligned16(scales)) return SDMI_ERR_ALIGNMENT;
+    if (rows == 0) return SDMI_OK;
+    MxElemArgs a = {};
+    a.x = x; a.ldx = ldx; a.rows = rows; a.K = K; a.codes = (unsigned char*)codes; a.scales = (unsigned char*)scales;
+    a.vec_in = vec_rows(x, ldx, t);
+    unsigned blocks;
+    if (!elem_grid(rows, K, &a.ktiles, &blocks)) return SDMI_ERR_BAD_ARG;
+    hipStream_t st = (hipStream_t)stream;
+    return t == 0 ? elem_launch<0, 0>(a, fmt, 0, blocks, st) : t == 1 ? elem_launch<1, 0>(a, fmt, 0, blocks, st) : elem_launch<2, 0>(a, fmt, 0, blocks, st);
+}
+
+extern "C" int sdmi_gated(const void* x, int64_t ldx, int64_t rows, int64_t inner, int32_t dtype, int32_t act, void* out,
+                          int32_t out_dtype, void* scales, int32_t fmt, void* stream) {
+    const int t = mx_src_type(dtype), to = fmt == SDMI_MX_NONE ? mx_src_type(out_dtype) : 0;
+    if (!x || !out || t < 0 || to < 0 || (act != 0 && act != 1) || (fmt != SDMI_MX_NONE && (!fmt_ok(fmt) || !scales)) ||
+        rows < 0 || inner <= 0 || inner > MX_MAX_K || ldx < 2 * inner || rows > MX_MAX_ROWS) return SDMI_ERR_BAD_ARG;
+    if (fmt != SDMI_MX_NONE && (!aligned16(out) || !aligned16(scales))) return SDMI_ERR_ALIGNMENT;
+    if (rows == 0) return SDMI_OK;
+    MxElemArgs a = {};
+    a.x = x; a.ldx = ldx; a.rows = rows; a.K = inner; a.codes = (unsigned char*)out; a.scales = (unsigned char*)scales;
+    a.out = out; a.ld_out = inner;
+    a.vec_in = vec_rows(x, ldx, t);
+    a.vec_gate = a.vec_in && inner % (t == 2 ? 4 : 8) == 0;
+    a.vec_out = vec_rows(out, inner, to);
+    unsigned blocks;
+    if (!elem_grid(rows, inner, &a.ktiles, &blocks)) return SDMI_ERR_BAD_ARG;
+    hipStream_t st = (hipStream_t)stream;
+    if (act == 0)
+        return t == 0 ? elem_launch<0, 1>(a, fmt, to, blocks, st) : t == 1 ? elem_launch<1, 1>(a, fmt, to, blocks, st) : elem_launch<2, 1>(a, fmt, to, blocks, st);
+    return t == 0 ? elem_launch<0, 2>(a, fmt, to, blocks, st) : t == 1 ? elem_launch<1, 2>(a, fmt, to, blocks, st) : elem_launch<2, 2>(a, fmt, to, blocks, st);
+}
+
+extern "C" int sdmi_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t K, int32_t fmt, void* out,
+                                  int64_t ld_out, int32_t out_dtype, void* stream) {
+    const int to = mx_src_type(out_dtype);
+    if (!codes || !scales || !out || to < 0 || !fmt_ok(fmt) || rows < 0 || K <= 0 || K > MX_MAX_K || ld_out < K || rows > MX_MAX_ROWS) return SDMI_ERR_BAD_ARG;
+    if (!aligned16(codes) || !aligned16(scales)) return SDMI_ERR_ALIGNMENT;
+    if (rows == 0) return SDMI_OK;
+    MxElemArgs a = {};
+    a.rows = rows; a.K = K; a.codes = (unsigned char*)codes; a.scales = (unsigned char*)scales; a.out = out; a.ld_out = ld_out;
+    a.vec_out = vec_rows(out, ld_out, to);
+    unsigned blocks;
+    if (!elem_grid(rows, K, &a.ktiles, &blocks)) return SDMI_ERR_BAD_ARG;
+    hipStream_t st = (hipStream_t)stream;
+#define SDMI_DQ(F, O) sdmi_mx_dequantise_kernel<F, O><<<blocks, 256, 0, st>>>(a)
+    if (fmt == SDMI_MX_FP8) { if (to == 0) SDMI_DQ(SDMI_MX_FP8, 0); else if (to == 1) SDMI_DQ(SDMI_MX_FP8, 1); else SDMI_DQ(SDMI_MX_FP8, 2); }
+    else { if (to == 0) SDMI_DQ(SDMI_MX_FP4, 0); else if (to == 1) SDMI_DQ(SDMI_MX_FP4, 1); else SDMI_DQ(SDMI_MX_FP4, 2); }
+#undef SDMI_DQ
+    SDMI_CHECK_LAUNCH();
+    return SDMI_OK;
+}
+
+template <int T, int FMT, int TO>
+static int norm_launch(const MxNormArgs& a, hipStream_t st) {
+    // 64 threads a row up to 1024 values (four rows a block), 256 above
+#define SDMI_NORM(TPR, U) sdmi_rmsnorm_kernel<T, FMT, TO, TPR, U><<<(unsigned)((a.rows + 256 / TPR - 1) / (256 / TPR)), 256, 0, st>>>(a)
+    if (a.C <= 512) SDMI_NORM(64, 1);
+    else if (a.C <= 1024) SDMI_NORM(64, 2);
+    else if (a.C <= 2048) SDMI_NORM(256, 1);
+    else if (a.C <= 4096) SDMI_NORM(256, 2);
+    else if (a.C <= 8192) SDMI_NORM(256, 4);
+    else SDMI_NORM(256, 8);
+#undef SDMI_NORM
+    SDMI_CHECK_LAUNCH();
+    return SDMI_OK;
+}
+
+template <int T> static int norm_type(const MxNormArgs& a, int fmt, int to, hipStream_t st) {
+    if (fmt == SDMI_MX_FP8) return norm_launch<T, SDMI_MX_FP8, 0>(a, st);
+    if (fmt == SDMI_MX_FP4) return norm_launch<T, SDMI_MX_FP4, 0>(a, st);
+    return to == 0 ? norm_launch<T, -1, 0>(a, st) : to == 1 ? norm_launch<T, -1, 1>(a, st) : norm_launch<T, -1, 2>(a, st);
+}
+
+extern "C" int sdmi_rmsnorm(const void* x, int64_t ldx, const void* res, int64_t ld_res, const float* gamma, float eps,
+                            int64_t rows, int64_t C, int32_t dtype, void* sum_out, void* out, int32_t out_dtype, void* scales,
+                            int32_t fmt, void* stream) {
+    const int t = mx_src_type(dtype), to = fmt == SDMI_MX_NONE ? mx_src_type(out_dtype) : 0;
+    if (!x || !gamma || !out || t < 0 || to < 0 || (fmt != SDMI_MX_NONE && (!fmt_ok(fmt) || !scales)) || rows < 0 || C <= 0 ||
+        C > SDMI_RMSNORM_MAX_C || ldx < C || (res && (ld_res < C || !sum_out)) || rows > MX_MAX_ROWS || !(eps >= 0.0f)) return SDMI_ERR_BAD_ARG;
+    if (!aligned16(gamma) || (fmt != SDMI_MX_NONE && (!aligned16(out) || !aligned16(scales)))) return SDMI_ERR_ALIGNMENT;
+    if (rows == 0) return SDMI_OK;
+    MxNormArgs a = {};
+    a.x = x; a.res = res; a.gamma = gamma; a.sum_out = res ? sum_out : nullptr; a.out = out;
+    a.codes = (unsigned char*)out; a.scales = (unsigned char*)scales;
+    a.ldx = ldx; a.ld_res = ld_res; a.rows = rows; a.C = C; a.eps = eps;
+    a.vec_x = vec_rows(x, ldx, t);
+    a.vec_res = res ? vec_rows(res, ld_res, t) : 0;
+    a.vec_out = C % 8 == 0 && (fmt != SDMI_MX_NONE || aligned16(out)) && (!a.sum_out || aligned16(a.sum_out));
+    hipStream_t st = (hipStream_t)stream;
+    return t == 0 ? norm_type<0>(a, fmt, to, st) : t == 1 ? norm_type<1>(a, fmt, to, st) : norm_type<2>(a, fmt, to, st);
+}

@@ -12,7 +12,9 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SDMI_LIB") or os.path.join(_HERE, "csrc", "libsdmi_hip.so")
 
 SDMI_OK = 0
-DTYPE_BF16, DTYPE_F16, DTYPE_F32_PLANES, DTYPE_F16_TO_BF16 = 0, 1, 2, 3
+DTYPE_BF16, DTYPE_F16, DTYPE_F32_PLANES, DTYPE_F16_TO_BF16, DTYPE_F32 = 0, 1, 2, 3, 4
+MX_NONE, MX_FP8, MX_FP4 = 0, 1, 2
+RMSNORM_MAX_C = 16384
 
 
 class SdmiError(RuntimeError):
@@ -52,7 +54,7 @@ class GemmArgs(C.Structure):
     ]
 
 
-ABI_VERSION = 13    # sdmi_abi_version() of the library this binding was written against (include/sdmi.h)
+ABI_VERSION = 14    # sdmi_abi_version() of the library this binding was written against (include/sdmi.h)
 
 _vp, _i32, _i64, _f32 = C.c_void_p, C.c_int32, C.c_int64, C.c_float
 
@@ -70,6 +72,17 @@ class XattnArgs(C.Structure):
         ("row_stats_out", C.c_void_p), ("row_stats_slots", C.c_int32),
         ("dtype", C.c_int32),
     ]
+
+
+class MxGemmArgs(C.Structure):
+    """sdmi_mx_gemm_args (include/sdmi.h)."""
+    _fields_ = [
+        ("x", C.c_void_p), ("x_codes", C.c_void_p), ("x_scales", C.c_void_p), ("w_codes", C.c_void_p), ("w_scales", C.c_void_p),
+        ("bias", C.c_void_p), ("res", C.c_void_p), ("out", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+        ("M", C.c_int64), ("N", C.c_int64), ("K", C.c_int64), ("ldx", C.c_int64), ("ld_res", C.c_int64), ("ld_out", C.c_int64),
+        ("x_dtype", C.c_int32), ("out_dtype", C.c_int32), ("fmt", C.c_int32), ("reserved", C.c_int32),
+    ]
+
 
 # name -> (restype, argtypes); every symbol include/sdmi.h declares
 SIGNATURES = {
@@ -122,6 +135,17 @@ SIGNATURES = {
     "sdmi_timestep_embedding": (C.c_int, [_vp, _vp, _i32, _i32, _f32, _i32, _vp]),
     "sdmi_ddim_step": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _f32, _f32, _f32, _f32, _f32, _i32, _vp]),
     "sdmi_image_to_u8": (C.c_int, [_vp, _vp, _i32, _i32, _i64, _vp]),
+    "sdmi_mx_codes_bytes": (_i64, [_i64, _i64, _i32]),
+    "sdmi_mx_scales_bytes": (_i64, [_i64, _i64]),
+    "sdmi_mx_quantize": (C.c_int, [_vp, _i64, _i64, _i64, _i32, _vp, _vp, _i32, _vp]),
+    "sdmi_mx_dequantize": (C.c_int, [_vp, _vp, _i64, _i64, _i32, _vp, _i64, _i32, _vp]),
+    "sdmi_rmsnorm": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _f32, _i64, _i64, _i32, _vp, _vp, _i32, _vp, _i32, _vp]),
+    "sdmi_gated": (C.c_int, [_vp, _i64, _i64, _i64, _i32, _i32, _vp, _i32, _vp, _i32, _vp]),
+    "sdmi_mx_weight_codes_bytes": (_i64, [_i64, _i64]),
+    "sdmi_mx_weight_scales_bytes": (_i64, [_i64, _i64]),
+    "sdmi_mx_pack_linear": (C.c_int, [_vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp]),
+    "sdmi_mx_gemm_workspace_bytes": (_i64, [C.POINTER(MxGemmArgs)]),
+    "sdmi_mx_gemm": (C.c_int, [C.POINTER(MxGemmArgs), _vp]),
     "sdmi_probe_mfma": (C.c_int, [_vp, _i32, C.POINTER(C.c_double), _vp]),
     "sdmi_probe_copy": (C.c_int, [_vp, _vp, _i64, _vp]),
 }

@@ -819,6 +819,271 @@ def layernorm(x, gamma, beta, eps=1e-5, out_dtype=None):
     return out
 
 
+# ----------------------------------------------------------------------------- block-scaled (MX) operators
+
+_MX_FMT = {"mxfp8": hip.MX_FP8, "mxfp4": hip.MX_FP4}
+_MX_DT = {BF16: hip.DTYPE_BF16, F16: hip.DTYPE_F16, torch.float32: hip.DTYPE_F32}
+
+
+class MxTensor:
+    """A matrix in block-scaled form: `shape` [..., K], `fmt` "mxfp8" (e4m3) or "mxfp4" (e2m1), and on the device the codes
+    and scales that include/sdmi.h lays out - `codes` uint8 [rows, bytes of a row], `scales` uint8 [ceil(K / 128), rows, 4].
+    Made by mx_quantize, rmsnorm and gated; read by linear_mx and mx_dequantize."""
+    __slots__ = ("codes", "scales", "fmt", "shape")
+
+    def __init__(self, codes, scales, fmt, shape):
+        self.codes, self.scales, self.fmt, self.shape = codes, scales, fmt, shape
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+class PackedMxWeight:
+    """[N, K] linear weights in 4 bits with one scale per 32 (sdmi_mx_pack_linear), and the fp32 bias or None."""
+    __slots__ = ("codes", "scales", "bias", "n_out", "k")
+
+    def __init__(self, codes, scales, bias, n_out, k):
+        self.codes, self.scales, self.bias, self.n_out, self.k = codes, scales, bias, n_out, k
+
+
+def _mx_fmt(fmt):
+    code = _MX_FMT.get(fmt)
+    if code is None:
+        raise hip.SdmiError(f"fmt must be 'mxfp8' or 'mxfp4', got {fmt!r}")
+    return code
+
+
+def _mx_dt(dtype, name):
+    code = _MX_DT.get(dtype)
+    if code is None:
+        raise hip.SdmiError(f"{name}: bf16, fp16 or fp32, not {dtype}")
+    return code
+
+
+def _mx_rows(t, name):
+    """(rows, columns, leading dimension) of [..., K] read as a matrix: unit inner stride, and rows one stride apart - a
+    column slice of a wider buffer is taken as it is."""
+    if not t.is_cuda:
+        raise hip.SdmiError(f"{name}: the HIP path needs device tensors (got {t.device}); there is no CPU fallback")
+    if t.dim() == 0 or t.shape[-1] == 0:
+        raise hip.SdmiError(f"{name}: needs a last axis of at least one value, got shape {tuple(t.shape)}")
+    k = t.shape[-1]
+    if t.is_contiguous():
+        return t.numel() // k, k, k
+    if t.numel() == 0:
+        return 0, k, k
+    if t.stride(-1) != 1 and k > 1:
+        raise hip.SdmiError(f"{name}: the last axis must have unit stride, got {t.stride()}")
+    ld = None
+    rows = 1
+    for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if n == 1:
+            continue
+        if ld is None:
+            ld = s
+        elif s != ld * rows:
+            raise hip.SdmiError(f"{name}: rows are not one stride apart (shape {tuple(t.shape)}, strides {t.stride()})")
+        rows *= n
+    ld = k if ld is None else ld
+    if ld < k:
+        raise hip.SdmiError(f"{name}: rows overlap (strides {t.stride()})")
+    return rows, k, ld
+
+
+def _mx_same(dev, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise hip.SdmiError(f"{name} is on {t.device}, the input on {dev}")
+
+
+class _on:
+    """The device of a tensor made current for a launch, and its current stream."""
+    __slots__ = ("index", "before")
+
+    def __init__(self, t):
+        self.index = t.device.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return _stream()
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+def _mx_empty(rows, k, fmt, shape, device):
+    steps = (k + 127) // 128
+    return MxTensor(torch.empty(rows, steps * (128 if fmt == "mxfp8" else 64), dtype=torch.uint8, device=device),
+                    torch.empty(steps, rows, 4, dtype=torch.uint8, device=device), fmt, shape)
+
+
+def mx_quantize(x, fmt="mxfp8"):
+    """x (bf16, fp16 or fp32, [..., K], rows may be strided) -> MxTensor: blocks of 32 along the last axis with a
+    power-of-two scale each (OCP Microscaling v1.0; a block with a NaN or an infinity becomes NaN)."""
+    code, dt = _mx_fmt(fmt), _mx_dt(x.dtype, "mx_quantize")
+    rows, k, ld = _mx_rows(x, "x")
+    q = _mx_empty(rows, k, fmt, x.shape, x.device)
+    if rows:
+        with _on(x) as st:
+            hip.check(hip.lib().sdmi_mx_quantize(x.data_ptr(), ld, rows, k, dt, q.codes.data_ptr(), q.scales.data_ptr(), code, st),
+                      "sdmi_mx_quantize")
+    return q
+
+
+def mx_dequantize(q, dtype=torch.float32):
+    """The values that an MxTensor stands for.  bf16 and fp32 hold them exactly (bf16 down to its subnormals); fp16 rounds."""
+    dt = _mx_dt(dtype, "mx_dequantize")
+    rows, k = q.codes.shape[0], q.shape[-1]
+    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    if rows:
+        with _on(out) as st:
+            hip.check(hip.lib().sdmi_mx_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), rows, k, _MX_FMT[q.fmt], out.data_ptr(),
+                                                   k, dt, st), "sdmi_mx_dequantize")
+    return out
+
+
+def rmsnorm(x, gamma, eps=1e-6, res=None, fmt=None, out_dtype=None):
+    """y = s / sqrt(mean(s^2) + eps) * gamma over the last axis, s = x + res (fp32).  x, res: bf16, fp16 or fp32 [..., C],
+    rows may be strided; gamma: fp32 [C]; C <= 16384.  y is a tensor of x's type (or out_dtype), or an MxTensor of `fmt` for
+    linear_mx.  Returns y, or with res (y, s), s stored in x's type: the new residual stream."""
+    dt = _mx_dt(x.dtype, "rmsnorm")
+    rows, c, ld = _mx_rows(x, "x")
+    if c > hip.RMSNORM_MAX_C:
+        raise hip.SdmiError(f"rmsnorm: rows of at most {hip.RMSNORM_MAX_C} values, got {c}")
+    _require(gamma, torch.float32, "gamma")
+    if gamma.numel() != c:
+        raise hip.SdmiError(f"rmsnorm: gamma has {gamma.numel()} values for rows of {c}")
+    if not eps >= 0.0:
+        raise hip.SdmiError(f"rmsnorm: eps must not be negative, got {eps}")
+    ld_res, s = 0, None
+    if res is not None:
+        if res.dtype != x.dtype or res.shape != x.shape:
+            raise hip.SdmiError(f"rmsnorm: res is {res.dtype} {tuple(res.shape)}, x {x.dtype} {tuple(x.shape)}")
+        ld_res = _mx_rows(res, "res")[2]
+        s = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _mx_same(x.device, gamma=gamma, res=res)
+    if fmt is None:
+        y = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
+        out, scales, code, odt = y.data_ptr(), None, hip.MX_NONE, _mx_dt(y.dtype, "rmsnorm out_dtype")
+    else:
+        if out_dtype is not None:
+            raise hip.SdmiError("rmsnorm: out_dtype goes with fmt=None")
+        code, odt = _mx_fmt(fmt), 0
+        y = _mx_empty(rows, c, fmt, x.shape, x.device)
+        out, scales = y.codes.data_ptr(), y.scales.data_ptr()
+    if rows:
+        with _on(x) as st:
+            hip.check(hip.lib().sdmi_rmsnorm(x.data_ptr(), ld, None if res is None else res.data_ptr(), ld_res, gamma.data_ptr(), eps,
+                                             rows, c, dt, None if s is None else s.data_ptr(), out, odt, scales, code, st),
+                      "sdmi_rmsnorm")
+    return y if res is None else (y, s)
+
+
+_GATES = {"gelu": 0, "silu": 1}
+
+
+def gated(x, act="gelu", fmt=None, out_dtype=None):
+    """a * act(b) for x = [a | b] along the last axis (the halves of a GEGLU or SwiGLU projection; act "gelu" is the erf form).
+    x: bf16, fp16 or fp32 [..., 2 I], rows may be strided.  Returns [..., I] in x's type (or out_dtype), or an MxTensor of `fmt`."""
+    dt = _mx_dt(x.dtype, "gated")
+    if act not in _GATES:
+        raise hip.SdmiError(f"gated: act must be 'gelu' or 'silu', got {act!r}")
+    rows, c2, ld = _mx_rows(x, "x")
+    if c2 % 2:
+        raise hip.SdmiError(f"gated: the last axis holds two halves, got {c2} columns")
+    c, shape = c2 // 2, torch.Size((*x.shape[:-1], c2 // 2))
+    if fmt is None:
+        y = torch.empty(shape, dtype=out_dtype or x.dtype, device=x.device)
+        out, scales, code, odt = y.data_ptr(), None, hip.MX_NONE, _mx_dt(y.dtype, "gated out_dtype")
+    else:
+        if out_dtype is not None:
+            raise hip.SdmiError("gated: out_dtype goes with fmt=None")
+        code, odt = _mx_fmt(fmt), 0
+        y = _mx_empty(rows, c, fmt, shape, x.device)
+        out, scales = y.codes.data_ptr(), y.scales.data_ptr()
+    if rows:
+        with _on(x) as st:
+            hip.check(hip.lib().sdmi_gated(x.data_ptr(), ld, rows, c, dt, _GATES[act], out, odt, scales, code, st), "sdmi_gated")
+    return y
+
+
+def pack_linear_mx(weight, bias=None):
+    """nn.Linear weight [N, K] (device tensor, fp32, bf16 or fp16) -> PackedMxWeight: quantised once to 4 bits with a scale per
+    32 values of K, in the order linear_mx reads them."""
+    if weight.dim() != 2 or weight.numel() == 0:
+        raise hip.SdmiError(f"pack_linear_mx: a weight is [N, K], got {tuple(weight.shape)}")
+    w = weight.detach()
+    dt = _mx_dt(w.dtype, "pack_linear_mx")
+    n, k, ld = _mx_rows(w, "weight")
+    b = None
+    if bias is not None:
+        b = _src(bias).clone()          # the packed layer owns its parameters: the caller's tensor may change
+        if b.shape != (n,):
+            raise hip.SdmiError(f"pack_linear_mx: bias {tuple(bias.shape)} for {n} outputs")
+    _mx_same(w.device, bias=b)
+    lib = hip.lib()
+    pw = PackedMxWeight(torch.empty(lib.sdmi_mx_weight_codes_bytes(n, k), dtype=torch.uint8, device=w.device),
+                        torch.empty(lib.sdmi_mx_weight_scales_bytes(n, k), dtype=torch.uint8, device=w.device), b, n, k)
+    with _on(w) as st:
+        hip.check(lib.sdmi_mx_pack_linear(w.data_ptr(), ld, n, k, dt, pw.codes.data_ptr(), pw.scales.data_ptr(), st),
+                  "sdmi_mx_pack_linear")
+    return pw
+
+
+@functools.lru_cache(maxsize=4096)
+def _mx_gemm_workspace(m, n, k, ldx, x_dt, fmt):
+    a = hip.MxGemmArgs()
+    a.M, a.N, a.K, a.ldx, a.x_dtype, a.fmt = m, n, k, ldx, x_dt, fmt
+    a.x = 16 if x_dt >= 0 else None          # (only whether there is one counts)
+    return hip.lib().sdmi_mx_gemm_workspace_bytes(C.byref(a))
+
+
+def linear_mx(x, pw, fmt=None, res=None, out_dtype=None):
+    """out = x @ W^T + bias + res with W in 4 bits (pack_linear_mx).  x: an MxTensor, or bf16 / fp16 / fp32 [..., K] that is
+    quantised to `fmt` (default "mxfp8") on the way.  out: [..., N] of out_dtype, by default x's type (bf16 for an MxTensor,
+    or res's type); res: [..., N] of that type."""
+    a = hip.MxGemmArgs()
+    if isinstance(x, MxTensor):
+        if fmt is not None and fmt != x.fmt:
+            raise hip.SdmiError(f"linear_mx: x is {x.fmt} already, fmt={fmt!r} was asked for")
+        m, k, ldx, x_dt, code = x.codes.shape[0], x.shape[-1], x.shape[-1], -1, _MX_FMT[x.fmt]
+        a.x_codes, a.x_scales = x.codes.data_ptr(), x.scales.data_ptr()
+        out_dtype = out_dtype or (res.dtype if res is not None else BF16)
+    else:
+        code, x_dt = _mx_fmt(fmt or "mxfp8"), _mx_dt(x.dtype, "linear_mx")
+        m, k, ldx = _mx_rows(x, "x")
+        a.x, a.ldx, a.x_dtype = x.data_ptr(), ldx, x_dt
+        out_dtype = out_dtype or x.dtype
+    if k != pw.k:
+        raise hip.SdmiError(f"linear_mx: K mismatch ({k} vs packed {pw.k})")
+    dev, n = x.device, pw.n_out
+    shape = torch.Size((*x.shape[:-1], n))
+    _mx_same(dev, weight=pw.codes, res=res)
+    a.out_dtype = _mx_dt(out_dtype, "linear_mx out_dtype")
+    if res is not None:
+        if res.dtype != out_dtype or res.shape != shape:
+            raise hip.SdmiError(f"linear_mx: res is {res.dtype} {tuple(res.shape)}, the output {out_dtype} {tuple(shape)}")
+        a.res, a.ld_res = res.data_ptr(), _mx_rows(res, "res")[2]
+    out = torch.empty(shape, dtype=out_dtype, device=dev)
+    if m == 0:
+        return out
+    a.M, a.N, a.K, a.fmt, a.ld_out = m, n, k, code, n
+    a.w_codes, a.w_scales, a.out = pw.codes.data_ptr(), pw.scales.data_ptr(), out.data_ptr()
+    if pw.bias is not None:
+        a.bias = pw.bias.data_ptr()
+    with _on(out) as st:
+        nbytes = _mx_gemm_workspace(m, n, k, ldx, x_dt, code)
+        if nbytes > 0:
+            ws = _scratch(nbytes, dev)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+        hip.check(hip.lib().sdmi_mx_gemm(C.byref(a), st), "sdmi_mx_gemm")
+    return out
+
+
 # ----------------------------------------------------------------------------- attention
 
 

@@ -1,0 +1,144 @@
+"""The block-scaled operators' refusals through the C ABI (every one returns before a kernel is launched) and the oracle they
+are checked against, on the CPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+import mx_oracle as O
+
+OK, BAD, ALIGN, WORKSPACE = 0, -1, -2, -3
+P = 4096            # stands for a device pointer: never read, the calls below are refused or empty
+DT = {"bf16": 0, "f16": 1, "f32": 4}
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from stablediffusion_amd import hip
+    return hip.lib()
+
+
+def test_quantise_refusals(lib):
+    q = lib.sdmi_mx_quantize
+    assert q(P, 64, 0, 64, 0, P, P, 1, None) == OK                     # no rows: an empty call
+    for bad in ((None, 64, 4, 64, 0, P, P, 1), (P, 64, 4, 64, 0, None, P, 1), (P, 64, 4, 64, 0, P, None, 1),
+                (P, 64, -1, 64, 0, P, P, 1), (P, 64, 4, 0, 0, P, P, 1), (P, 63, 4, 64, 0, P, P, 1), (P, 64, 4, 64, 2, P, P, 1),
+                (P, 64, 4, 64, 3, P, P, 1), (P, 64, 4, 64, 0, P, P, 0), (P, 64, 4, 64, 0, P, P, 3), (P, 1 << 25, 4, (1 << 24) + 1, 0, P, P, 1),
+                (P, 64, 1 << 31, 64, 0, P, P, 1)):
+        assert q(*bad, None) == BAD, bad
+    assert q(P, 64, 4, 64, 0, P + 8, P, 1, None) == ALIGN
+    assert q(P, 64, 4, 64, 0, P, P + 4, 2, None) == ALIGN
+
+
+def test_dequantise_refusals(lib):
+    d = lib.sdmi_mx_dequantize
+    assert d(P, P, 0, 64, 1, P, 64, 0, None) == OK
+    for bad in ((None, P, 4, 64, 1, P, 64, 0), (P, None, 4, 64, 1, P, 64, 0), (P, P, 4, 64, 1, None, 64, 0), (P, P, 4, 64, 0, P, 64, 0),
+                (P, P, 4, 64, 1, P, 63, 0), (P, P, 4, 0, 1, P, 64, 0), (P, P, -4, 64, 1, P, 64, 0), (P, P, 4, 64, 1, P, 64, 2)):
+        assert d(*bad, None) == BAD, bad
+    assert d(P + 2, P, 4, 64, 1, P, 64, 0, None) == ALIGN
+
+
+def test_rmsnorm_refusals(lib):
+    n = lib.sdmi_rmsnorm
+    good = [P, 64, P, 64, P, 1e-6, 0, 64, 0, P, P, 0, P, 1]
+    assert n(*good, None) == OK
+    for i, v in ((0, None), (1, 63), (3, 63), (4, None), (5, -1.0), (5, float("nan")), (6, -1), (7, 0), (7, 16385), (8, 2), (9, None),
+                 (10, None), (12, None), (13, 3)):
+        a = list(good)
+        a[i] = v
+        a[6] = 4 if i != 6 else a[6]
+        if i == 7 and v > 64:
+            a[1] = a[3] = v
+        assert n(*a, None) == BAD, (i, v)
+    a = list(good)
+    a[6], a[13], a[11] = 4, 0, 2                                        # plain result of an unknown type
+    assert n(*a, None) == BAD
+    for i in (4, 10, 12):
+        a = list(good)
+        a[6], a[i] = 4, P + 4
+        assert n(*a, None) == ALIGN, i
+
+
+def test_gated_refusals(lib):
+    g = lib.sdmi_gated
+    good = [P, 128, 0, 64, 0, 0, P, 0, P, 1]
+    assert g(*good, None) == OK
+    for i, v in ((0, None), (1, 127), (2, -1), (3, 0), (4, 3), (5, 2), (5, -1), (6, None), (8, None), (9, 7)):
+        a = list(good)
+        a[i] = v
+        a[2] = 4 if i != 2 else a[2]
+        assert g(*a, None) == BAD, (i, v)
+    a = list(good)
+    a[2], a[6] = 4, P + 2
+    assert g(*a, None) == ALIGN
+
+
+def test_pack_refusals(lib):
+    p = lib.sdmi_mx_pack_linear
+    for bad in ((None, 64, 8, 64, 4, P, P), (P, 64, 8, 64, 4, None, P), (P, 64, 8, 64, 4, P, None), (P, 63, 8, 64, 4, P, P),
+                (P, 64, 0, 64, 4, P, P), (P, 64, 8, 0, 4, P, P), (P, 64, 8, 64, 2, P, P), (P, 64, (1 << 24) + 1, 64, 4, P, P)):
+        assert p(*bad, None) == BAD, bad
+    assert p(P, 64, 8, 64, 4, P + 1, P, None) == ALIGN
+
+
+def _gemm(**kw):
+    from stablediffusion_amd import hip
+    a = hip.MxGemmArgs()
+    base = dict(x=P, ldx=64, x_dtype=0, w_codes=P, w_scales=P, out=P, M=0, N=64, K=64, ld_out=64, out_dtype=0, fmt=1)
+    for k, v in {**base, **kw}.items():
+        setattr(a, k, v)
+    return a
+
+
+def test_product_refusals(lib):
+    g = lambda **kw: lib.sdmi_mx_gemm(C.byref(_gemm(**kw)), None)
+    assert g() == OK
+    assert g(x=None, x_codes=P, x_scales=P) == OK
+    for bad in (dict(w_codes=None), dict(w_scales=None), dict(out=None), dict(x=None), dict(x=None, x_codes=P), dict(ldx=63), dict(x_dtype=3),
+                dict(N=0), dict(K=0), dict(M=-1), dict(fmt=0), dict(out_dtype=2), dict(ld_out=63), dict(res=P, ld_res=63), dict(K=(1 << 24) + 1, ldx=1 << 25)):
+        assert g(**{"M": 4, **bad}) == BAD, bad
+    assert lib.sdmi_mx_gemm(None, None) == BAD
+    for bad in (dict(w_codes=P + 8), dict(w_scales=P + 2), dict(x=None, x_codes=P + 8, x_scales=P)):
+        assert g(M=4, **bad) == ALIGN, bad
+    need = lib.sdmi_mx_gemm_workspace_bytes(C.byref(_gemm(M=300, K=1000, ldx=1000)))
+    assert need > 0
+    assert g(M=300, K=1000, ldx=1000) == WORKSPACE
+    assert g(M=300, K=1000, ldx=1000, workspace=P, workspace_bytes=need - 1) == WORKSPACE
+    assert g(M=300, K=1000, ldx=1000, workspace=P + 4, workspace_bytes=need) == WORKSPACE
+    assert lib.sdmi_mx_gemm_workspace_bytes(C.byref(_gemm(M=4, K=0))) == -1
+
+
+def test_sizes(lib):
+    assert lib.sdmi_mx_codes_bytes(3, 129, 1) == 3 * 256 and lib.sdmi_mx_codes_bytes(3, 129, 2) == 3 * 128
+    assert lib.sdmi_mx_scales_bytes(3, 129) == 2 * 3 * 4
+    assert lib.sdmi_mx_codes_bytes(3, 0, 1) == lib.sdmi_mx_scales_bytes(-1, 4) == lib.sdmi_mx_codes_bytes(3, 4, 0) == -1
+    assert lib.sdmi_mx_weight_codes_bytes(65, 129) == 2 * 2 * 4096 and lib.sdmi_mx_weight_scales_bytes(65, 129) == 2 * 2 * 256
+
+
+def test_python_refusals_need_no_gpu():
+    from stablediffusion_amd import hip, ops
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    for call in (lambda: ops.mx_quantize(x), lambda: ops.rmsnorm(x, torch.ones(64)), lambda: ops.gated(x), lambda: ops.pack_linear_mx(x),
+                 lambda: ops.mx_quantize(x, "fp8"), lambda: ops.gated(x, act="relu"), lambda: ops.mx_quantize(x.to(torch.int8))):
+        with pytest.raises(hip.SdmiError):
+            call()
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
+def test_oracle_against_the_formats_own_tables(fmt):
+    """Every value that the oracle gives is scale times a representable element, and no representable element is nearer."""
+    emax, emin, digits, most = O.FORMATS[fmt]
+    table = {0.0}
+    for e in range(emin, emax + 1):
+        for m in range(2 ** digits):
+            table.add((1 + m / 2 ** digits) * 2.0 ** e)
+            table.add(m / 2 ** digits * 2.0 ** emin)
+    table = torch.tensor(sorted(t for t in table if t <= most), dtype=torch.float64)
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(16, 96, generator=g, dtype=torch.float64) * torch.exp(4 * torch.randn(16, 1, generator=g, dtype=torch.float64))
+    scale = O.power(O.scale_exponents(x, fmt)).repeat_interleave(32, dim=1)
+    got, want = O.values(x, fmt) / scale, (x / scale).clamp(-most, most)
+    far = (got.abs()[..., None] - table).abs().amin(-1)
+    assert float(far.max()) == 0.0
+    assert bool(((got - want).abs() <= (want.abs()[..., None] - table).abs().amin(-1)).all())
