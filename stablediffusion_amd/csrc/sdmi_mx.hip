@@ -60,9 +60,9 @@ __global__ __launch_bounds__(256) void sdmi_mx_elem_kernel(MxElemArgs p) {
             const unsigned dw = mx_quantise8<FMT>(f[s], lane, c);
             if (row < p.rows) {
                 if constexpr (FMT == SDMI_MX_FP8)
-                    *reinterpret_cast<uint2*>(p.codes + row * nsteps * 128 + k0) = c;
+                    *reinterpret_cast<uint2*>(p.codes + ((step * 2 + (sub >> 3)) * p.rows + row) * 64 + (sub & 7) * 8) = c;
                 else
-                    *reinterpret_cast<unsigned*>(p.codes + row * nsteps * 64 + (k0 >> 1)) = c.x;
+                    *reinterpret_cast<unsigned*>(p.codes + (step * p.rows + row) * 64 + sub * 4) = c.x;
                 if (sub == 0) *reinterpret_cast<unsigned*>(p.scales + (step * p.rows + row) * 4) = dw;
             }
         }
@@ -83,8 +83,8 @@ __global__ __launch_bounds__(256) void sdmi_mx_dequantise_kernel(MxElemArgs p) {
     for (int s = 0; s < EL_STEPS; ++s) {
         const int64_t step = (int64_t)tile_k * EL_STEPS + s;
         if (step >= nsteps) break;
-        if constexpr (FMT == SDMI_MX_FP8) c[s] = *reinterpret_cast<const uint2*>(p.codes + row * nsteps * 128 + step * 128 + sub * 8);
-        else c[s].x = *reinterpret_cast<const unsigned*>(p.codes + row * nsteps * 64 + step * 64 + sub * 4);
+        if constexpr (FMT == SDMI_MX_FP8) c[s] = *reinterpret_cast<const uint2*>(p.codes + ((step * 2 + (sub >> 3)) * p.rows + row) * 64 + (sub & 7) * 8);
+        else c[s].x = *reinterpret_cast<const unsigned*>(p.codes + (step * p.rows + row) * 64 + sub * 4);
         sc[s] = p.scales[(step * p.rows + row) * 4 + (sub >> 2)];
     }
 #pragma unroll
@@ -193,9 +193,9 @@ __global__ __launch_bounds__(256) void sdmi_rmsnorm_kernel(MxNormArgs p) {
             const unsigned dw = mx_quantise8<FMT>(gm, lane, c);
             if (row < p.rows) {
                 if constexpr (FMT == SDMI_MX_FP8)
-                    *reinterpret_cast<uint2*>(p.codes + row * nsteps * 128 + c0) = c;
+                    *reinterpret_cast<uint2*>(p.codes + (c0 / 64 * p.rows + row) * 64 + (c0 & 63)) = c;
                 else
-                    *reinterpret_cast<unsigned*>(p.codes + row * nsteps * 64 + (c0 >> 1)) = c.x;
+                    *reinterpret_cast<unsigned*>(p.codes + (step * p.rows + row) * 64 + ((c0 & 127) >> 1)) = c.x;
                 if ((lane & 15) == 0) *reinterpret_cast<unsigned*>(p.scales + (step * p.rows + row) * 4) = dw;
             }
         }

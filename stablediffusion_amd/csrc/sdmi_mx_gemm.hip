@@ -10,6 +10,7 @@
 // column 16 g + 4 f + r of its group: the four accumulator quads of a lane are then 16 CONSECUTIVE columns, stored as two
 // 16-byte vectors, and the four lanes of a token write a whole 128-byte line.
 #include "sdmi_mx.h"
+#include <type_traits>
 
 typedef __attribute__((ext_vector_type(8))) int i32x8;
 
@@ -53,8 +54,10 @@ struct MxGemmDev {
     const float* bias;
     const void* res;
     void* out;
-    int64_t M, N, ksteps, ld_res, ld_out;
-    int type, vec_out;         // of out and res: 0 bf16, 1 f16, 2 fp32
+    const void* x;             // the direct form that quantises: plain activations
+    int64_t M, N, K, ksteps, ldx, ld_res, ld_out;
+    int vec_x, vec_out;
+    int type;                  // of out and res: 0 bf16, 1 f16, 2 fp32
 };
 
 __device__ __forceinline__ i32x8 mx_op4(const uint4& a) { return (i32x8){(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0}; }
@@ -95,48 +98,404 @@ __device__ __forceinline__ void mx_store_quad(const MxGemmDev& p, int64_t m, int
     }
 }
 
-// Few rows: a workgroup takes one weight fragment (16 columns) and MT x 16 tokens; its four waves take every fourth k-step
-// straight from memory into registers and join their sums through LDS in a fixed order.
-template <int FMT, int MT>
-__global__ __launch_bounds__(256) void sdmi_mx_direct_kernel(MxGemmDev p) {
-    __shared__ f32x4 part[4][MT][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, q = lane >> 4;
-    const int64_t grp = blockIdx.x >> 2, m0 = (int64_t)blockIdx.y * (16 * MT);
-    const int frag = blockIdx.x & 3;
-    constexpr int RB = FMT == SDMI_MX_FP8 ? 128 : 64;      // bytes of a row's k-step
-    const unsigned char* const wc = p.wc + grp * p.ksteps * 4096 + frag * 1024 + lane * 16;
-    const unsigned char* const ws = p.ws + grp * p.ksteps * 256 + lane * 4 + frag;
-    const unsigned char* xc[MT];
-    int64_t xr[MT];
-    f32x4 acc[MT];
+// out[m, n .. n + 16): the four quads of a lane are consecutive columns
+__device__ __forceinline__ void mx_store_run(const MxGemmDev& p, int64_t m, int64_t n, const f32x4* v) {
+    if (m >= p.M) return;
+    if (!p.vec_out || n + 16 > p.N) {
 #pragma unroll
-    for (int mi = 0; mi < MT; ++mi) {
-        xr[mi] = min(m0 + mi * 16 + row, p.M - 1);
-        xc[mi] = p.xc + xr[mi] * p.ksteps * RB + q * 16;
-        acc[mi] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int f = 0; f < 4; ++f) mx_store_quad(p, m, n + 4 * f, v[f]);
+        return;
     }
-    for (int64_t s = wave; s < p.ksteps; s += 4) {
-        const uint4 w = *reinterpret_cast<const uint4*>(wc + s * 4096);
-        const int wsc = ws[s * 256];
+    float a[16];
 #pragma unroll
-        for (int mi = 0; mi < MT; ++mi) {
-            const int xsc = p.xs[(s * p.M + xr[mi]) * 4 + q];
-            const uint4 a = *reinterpret_cast<const uint4*>(xc[mi] + s * RB);
-            if constexpr (FMT == SDMI_MX_FP8) {
-                const uint4 b = *reinterpret_cast<const uint4*>(xc[mi] + s * RB + 64);
-                acc[mi] = mx_mfma<FMT, 0>(mx_op4(w), mx_op8(a, b), acc[mi], wsc, xsc);
-            } else {
-                acc[mi] = mx_mfma<FMT, 0>(mx_op4(w), mx_op4(a), acc[mi], wsc, xsc);
-            }
+    for (int f = 0; f < 4; ++f)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) a[4 * f + r] = v[f][r];
+    if (p.bias) {
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+            const f32x4 b = *reinterpret_cast<const f32x4*>(p.bias + n + 4 * f);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) a[4 * f + r] += b[r];
         }
     }
 #pragma unroll
-    for (int mi = 0; mi < MT; ++mi) part[wave][mi][lane] = acc[mi];
-    __syncthreads();
-    for (int mi = wave; mi < MT; mi += 4) {
-        const f32x4 v = (part[0][mi][lane] + part[1][mi][lane]) + (part[2][mi][lane] + part[3][mi][lane]);
-        mx_store_quad(p, m0 + mi * 16 + row, grp * 64 + 16 * q + 4 * frag, v);
+    for (int h = 0; h < 2; ++h) {
+        float b[8];
+        if (p.type == 2) {
+            if (p.res) {
+                mx_load8<2>(reinterpret_cast<const float*>(p.res) + m * p.ld_res + n + 8 * h, 8, true, b);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) a[8 * h + j] += b[j];
+            }
+            mx_store8<2>(reinterpret_cast<float*>(p.out) + m * p.ld_out + n + 8 * h, 8, true, a + 8 * h);
+        } else {
+            if (p.res) {
+                const uint4 r = *reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned short*>(p.res) + m * p.ld_res + n + 8 * h);
+                if (p.type == 0) elem_unpack8<0>(r, b); else elem_unpack8<1>(r, b);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) a[8 * h + j] += b[j];
+            }
+            *reinterpret_cast<uint4*>(reinterpret_cast<unsigned short*>(p.out) + m * p.ld_out + n + 8 * h) =
+                p.type == 0 ? elem_pack8<0>(a + 8 * h) : elem_pack8<1>(a + 8 * h);
+        }
     }
+}
+
+// ---- direct form --------------------------------------------------------------------------------------------------------
+// Few tokens: the weights' bytes are the work, and a workgroup has to have many of them in flight.  It takes NF of a group's
+// four fragments (4 NF columns of every 16) for MT x 16 tokens; its KW waves take every KW-th k-step from memory straight into
+// registers, U k-steps ahead of the ones they multiply, and join their sums through LDS in a fixed order.
+// SRC >= 0: x is a plain matrix of that type (mx_src_type) and at most MX_FUSED_ROWS rows, which every workgroup quantises for
+// itself into LDS while its first weights are on their way: one launch instead of two.
+constexpr int MX_FUSED_ROWS = 4;
+
+template <int FMT, int MT, int NF, int KW, int U, int SRC>
+__global__ __launch_bounds__(64 * KW) void sdmi_mx_direct_kernel(MxGemmDev p) {
+    extern __shared__ unsigned char smem[];
+    constexpr int RB = FMT == SDMI_MX_FP8 ? 128 : 64;      // bytes of a row's k-step
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = lane & 15, q = lane >> 4;
+    constexpr int PARTS = 4 / NF;
+    const int64_t grp = blockIdx.x / PARTS, m0 = (int64_t)blockIdx.y * (16 * MT);
+    const int f0 = (int)(blockIdx.x % PARTS) * NF;
+    const int nk = (int)p.ksteps, mine = (nk - wave + KW - 1) / KW;                 // k-steps of this wave (<= 0: none)
+    const unsigned char* const wc = p.wc + (grp * p.ksteps + wave) * 4096 + f0 * 1024 + lane * 16;
+    const unsigned char* const ws = p.ws + (grp * p.ksteps + wave) * 256 + lane * 4;
+    const unsigned char* xc[MT];
+    const unsigned char* xs[MT];
+    f32x4 acc[MT][NF];
+#pragma unroll
+    for (int mi = 0; mi < MT; ++mi) {
+        const int64_t r = min(m0 + mi * 16 + row, p.M - 1);
+        if constexpr (SRC < 0) {
+            xc[mi] = p.xc + (wave * (RB / 64) * p.M + r) * 64 + q * 16;
+            xs[mi] = p.xs + (wave * p.M + r) * 4 + q;
+        }
+#pragma unroll
+        for (int f = 0; f < NF; ++f) acc[mi][f] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+    uint4 w[2][U][NF], a[2][U][SRC < 0 ? MT : 1], b[2][U][SRC < 0 && FMT == SDMI_MX_FP8 ? MT : 1];
+    int wsc[2][U], xsc[2][U][SRC < 0 ? MT : 1];
+    auto load = [&](int buf, int i0) {                     // k-steps i0 .. i0 + U of this wave (past the end: the last one again)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t at = (int64_t)min(i0 + u, mine - 1) * KW;
+#pragma unroll
+            for (int f = 0; f < NF; ++f) w[buf][u][f] = *reinterpret_cast<const uint4*>(wc + at * 4096 + f * 1024);
+            wsc[buf][u] = *reinterpret_cast<const int*>(ws + at * 256);
+            if constexpr (SRC < 0) {
+#pragma unroll
+                for (int mi = 0; mi < MT; ++mi) {
+                    a[buf][u][mi] = *reinterpret_cast<const uint4*>(xc[mi] + at * p.M * RB);
+                    if constexpr (FMT == SDMI_MX_FP8) b[buf][u][mi] = *reinterpret_cast<const uint4*>(xc[mi] + at * p.M * RB + p.M * 64);
+                    xsc[buf][u][mi] = xs[mi][at * p.M * 4];
+                }
+            }
+        }
+    };
+    if (mine > 0) load(0, 0);
+    unsigned char* const own = smem;                       // SRC >= 0: [nk][M][RB] codes, then [nk][M][4] scales
+    const int rows = (int)p.M;
+    unsigned char* const own_s = smem + nk * rows * RB;
+    if constexpr (SRC >= 0) {
+        // the wave quantises the k-steps that it alone will read: four (k-step, row) pairs at a time, 16 lanes each, and AT
+        // times four on their way together (pairs past the end: the last one again)
+        constexpr int AT = 4;
+        const typename MxElem<SRC>::type* const x = reinterpret_cast<const typename MxElem<SRC>::type*>(p.x);
+        const int pairs = mine * rows;
+        for (int i0 = 0; i0 < pairs; i0 += 4 * AT) {
+            float f[AT][8];
+            int at[AT];
+#pragma unroll
+            for (int u = 0; u < AT; ++u) {
+                const int j = min(i0 + 4 * u + q, pairs - 1), step = wave + (j / rows) * KW, r = j % rows;
+                const int64_t k0 = (int64_t)step * MX_KSTEP + row * 8;
+                at[u] = step * rows + r;
+                mx_load8<SRC>(x + r * p.ldx + k0, (int)max((int64_t)0, min((int64_t)8, p.K - k0)), p.vec_x, f[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < AT; ++u) {
+                uint2 c;
+                const unsigned dw = mx_quantise8<FMT>(f[u], lane, c);
+                if constexpr (FMT == SDMI_MX_FP8) *reinterpret_cast<uint2*>(own + at[u] * RB + row * 8) = c;
+                else *reinterpret_cast<unsigned*>(own + at[u] * RB + row * 4) = c.x;
+                if (row == 0) *reinterpret_cast<unsigned*>(own_s + at[u] * 4) = dw;
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // other lanes of this wave read them
+    }
+    auto multiply = [&](int buf, int i0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i0 + u >= mine) break;                     // (uniform)
+#pragma unroll
+            for (int mi = 0; mi < MT; ++mi) {
+                i32x8 x;
+                int sc;
+                if constexpr (SRC < 0) {
+                    if constexpr (FMT == SDMI_MX_FP8) x = mx_op8(a[buf][u][mi], b[buf][u][mi]);
+                    else x = mx_op4(a[buf][u][mi]);
+                    sc = xsc[buf][u][mi];
+                } else {
+                    const int at = (wave + (i0 + u) * KW) * rows + min(row, rows - 1);
+                    const uint4 lo = *reinterpret_cast<const uint4*>(own + at * RB + q * 16);
+                    if constexpr (FMT == SDMI_MX_FP8) x = mx_op8(lo, *reinterpret_cast<const uint4*>(own + at * RB + q * 16 + 64));
+                    else x = mx_op4(lo);
+                    sc = own_s[at * 4 + q];
+                }
+                const int s4 = wsc[buf][u] >> (8 * f0);
+#pragma unroll
+                for (int f = 0; f < NF; ++f) acc[mi][f] = mx_mfma_f<FMT>(f, mx_op4(w[buf][u][f]), x, acc[mi][f], s4, sc);
+            }
+        }
+    };
+    for (int i = 0; i < mine; i += 2 * U) {
+        if (i + U < mine) load(1, i + U);
+        multiply(0, i);
+        if (i + 2 * U < mine) load(0, i + 2 * U);
+        if (i + U < mine) multiply(1, i + U);
+    }
+    if constexpr (SRC >= 0) __syncthreads();               // the codes' place becomes that of the sums
+    f32x4* const part = reinterpret_cast<f32x4*>(smem);
+#pragma unroll
+    for (int mi = 0; mi < MT; ++mi)
+#pragma unroll
+        for (int f = 0; f < NF; ++f) part[((wave * MT + mi) * NF + f) * 64 + lane] = acc[mi][f];
+    __syncthreads();
+    for (int t = wave; t < MT * NF; t += KW) {
+        f32x4 v = part[t * 64 + lane];
+#pragma unroll
+        for (int k = 1; k < KW; ++k) v += part[(k * MT * NF + t) * 64 + lane];
+        mx_store_quad(p, m0 + t / NF * 16 + row, grp * 64 + 16 * q + 4 * (f0 + t % NF), v);
+    }
+}
+
+// ---- tiled form ---------------------------------------------------------------------------------------------------------
+// A workgroup computes BM tokens x 64 WGN columns; wave (wm, wn) MF x 16 tokens x one group of 64 columns.  A k-step's codes
+// and scales come through a ring of ST LDS stages, filled by LDS-DMA: weights and their scales as they lie in memory, rows of
+// activations with their 16-byte chunks exchanged (chunk c of row r lies at c ^ swizzle(r)), so that the 16 rows of a fragment
+// read meet no bank twice - an LDS-DMA writes in lane order, so the exchange is made on the side of the global address.
+// One barrier a k-step, in its middle.
+// `mask`: the lanes that load, all or none.  A fill past the last k-step is issued with none: it moves nothing and still counts
+// as issued and landed, so that every k-step waits for the same number of instructions and the loop has no branch.
+#define MX_GLDS(NAME, OP)                                                                                            \
+    __device__ __forceinline__ void NAME(unsigned d0, const void* sb, unsigned v0, unsigned mask) {                   \
+        unsigned keep;                                                                                               \
+        uint64_t all;                                                                                                \
+        asm volatile(SDMI_M0_SAVE "s_mov_b32 m0, %[d0]\n\ts_mov_b64 %[all], exec\n\ts_mov_b32 exec_lo, %[mask]\n\ts_mov_b32 exec_hi, %[mask]\n\ts_nop 0\n\t"  \
+                     OP " %[v0], %[sb]\n\ts_mov_b64 exec, %[all]\n\t" SDMI_M0_REST                                   \
+                     : [keep] "=&s"(keep), [all] "=&s"(all)                                                          \
+                     : [d0] "s"(d0), [sb] "s"(sb), [v0] "v"(v0), [mask] "s"(__builtin_amdgcn_readfirstlane(mask))                                    \
+                     : "memory");                                                                                    \
+    }
+MX_GLDS(mx_glds16, "global_load_lds_dwordx4")
+MX_GLDS(mx_glds4, "global_load_lds_dword")
+
+// all but the youngest N fill instructions have landed, and so have the LDS reads
+template <int N> __device__ __forceinline__ void mx_wait() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory"); }
+
+template <int FMT, int BM, int WGM, int WGN, int ST> struct MxTile {
+    static constexpr int RB = FMT == SDMI_MX_FP8 ? 128 : 64;                     // bytes of a row's k-step
+    static constexpr int NW = WGM * WGN, THREADS = 64 * NW, BN = 64 * WGN, MF = BM / WGM / 16;
+    static constexpr int HALF = MF / 2, HR = HALF * 16;                          // fragments and rows of a wave's half
+    static constexpr int XJ = (BM / 2 + 63) / 64;                                // scale instructions of a half
+    static constexpr int A_BYTES = BM * RB, W_BYTES = WGN * 4096, AS_BYTES = 2 * XJ * 256, WS_BYTES = WGN * 256;
+    static constexpr int STAGE = A_BYTES + W_BYTES + AS_BYTES + WS_BYTES;
+    static constexpr int AI = A_BYTES / 1024 / NW, WI = W_BYTES / 1024 / NW;     // LDS-DMA instructions of a wave and stage
+    static constexpr int SJ = 2 * XJ + WGN, SI = (SJ + NW - 1) / NW;             // scale instructions: the halves', one a group
+    static constexpr int PER = AI + WI + SI, LDS = STAGE * ST;
+    static_assert(A_BYTES % (1024 * NW) == 0 && W_BYTES % (1024 * NW) == 0 && MF % 2 == 0 && MF * 16 * WGM == BM, "tile");
+    static_assert(AI % 2 == 0 || AI == 1, "halves");
+    static_assert((ST - 1) * PER < 64 && LDS <= 160 * 1024, "ring");
+};
+
+template <int FMT, int BM, int WGM, int WGN, int ST>
+__global__ __launch_bounds__(64 * WGM * WGN, 2) void sdmi_mx_tiled_kernel(MxGemmDev p) {
+    typedef MxTile<FMT, BM, WGM, WGN, ST> T;
+    extern __shared__ unsigned char smem[];
+    const unsigned lds_base = (unsigned)(size_t)(__attribute__((address_space(3))) unsigned char*)smem;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WGN, wn = wave % WGN, row = lane & 15, q = lane >> 4;
+
+    // Workgroups go round the 8 XCDs; each XCD takes a run of consecutive tiles, and a run walks 8 token tiles before the next
+    // column tile, so that the tiles an XCD works on together share their operands in its L2.
+    const unsigned tm = (unsigned)((p.M + BM - 1) / BM), tn = (unsigned)((p.N + T::BN - 1) / T::BN), total = tm * tn;
+    const unsigned xcd = blockIdx.x & 7, each = total >> 3, more = total & 7;
+    const unsigned id = (xcd < more ? xcd * (each + 1) : more + xcd * each) + (blockIdx.x >> 3);
+    const unsigned band = id / (8 * tn), height = min(8u, tm - band * 8), in_band = id - band * 8 * tn;
+    const int64_t m0 = (int64_t)(band * 8 + in_band % height) * BM;
+    const int64_t g0 = (int64_t)(in_band / height) * WGN, groups = (p.N + 63) >> 6;
+
+    const int nk = (int)p.ksteps;
+
+    // Fills.  A wave's tokens are two halves of HR rows: with the weights go the first halves ("X" of a stage), the second
+    // halves ("Y") follow half a k-step later, as they are read, so that each place in the ring is free again half a k-step
+    // earlier than it would be as a whole and the fills run ST - 1 / 2 k-steps ahead.
+    // Row j of X is row j % HR of the first half of wave row j / HR.  Per-lane offsets are constant over the k-steps.
+    auto tile_row = [](int j, bool y) { return j / T::HR * (2 * T::HR) + j % T::HR + (y ? T::HR : 0); };
+    const int64_t a_step = p.M * T::RB;
+    unsigned a_off[T::AI], w_off[T::WI], s_off[T::SI], a_dst[T::AI], s_dst[T::SI];
+    int64_t a_add[T::AI];
+    bool a_y[T::AI], s_y[T::SI];
+    const unsigned char* s_src[T::SI];
+    int64_t s_step[T::SI];
+#pragma unroll
+    for (int i = 0; i < T::AI; ++i) {
+        a_y[i] = T::AI == 1 ? wave >= T::NW / 2 : i >= T::AI / 2;                // an instruction takes 16 rows of a plane
+        const int c = T::AI == 1 ? wave % (T::NW / 2) : (i % (T::AI / 2)) * T::NW + wave, plane = c / (BM / 32);
+        const int first = tile_row(c % (BM / 32) * 16, a_y[i]), r = first + (lane >> 2);
+        const int64_t rr = min((int64_t)r, p.M - 1 - m0);                        // rows past the end repeat the last one
+        a_off[i] = (unsigned)rr * 64 + ((lane & 3) ^ ((r >> 1) & 3)) * 16;
+        a_add[i] = plane * p.M * 64 - (a_y[i] ? a_step : 0);
+        a_dst[i] = (plane * BM + first) * 64;
+    }
+#pragma unroll
+    for (int i = 0; i < T::WI; ++i) {
+        const int c = i * T::NW + wave;
+        const int64_t g = min((int64_t)(c >> 2), groups - 1 - g0);
+        w_off[i] = (unsigned)(g * p.ksteps * 4096) + (c & 3) * 1024 + lane * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < T::SI; ++i) {
+        const int job = (i * T::NW + wave) % T::SJ;                              // (a job done twice writes the same bytes twice)
+        s_y[i] = job >= T::XJ && job < 2 * T::XJ;
+        s_dst[i] = T::A_BYTES + T::W_BYTES + job * 256;
+        if (job < 2 * T::XJ) {
+            const int jr = (job % T::XJ * 64 + lane) % (BM / 2);
+            const int64_t r = min(m0 + tile_row(jr, s_y[i]), p.M - 1);
+            s_off[i] = (unsigned)((r - m0) * 4);
+            s_src[i] = p.xs + m0 * 4;
+            s_step[i] = p.M * 4;
+        } else {
+            const int64_t g = min(g0 + (job - 2 * T::XJ), groups - 1);
+            s_off[i] = lane * 4;
+            s_src[i] = p.ws + g * p.ksteps * 256;
+            s_step[i] = 256;
+        }
+        if (s_y[i]) s_src[i] -= s_step[i];
+    }
+    const unsigned char* a_src = p.xc + m0 * 64;
+    const unsigned char* w_src = p.wc + g0 * p.ksteps * 4096;
+    // Instruction j of the PER of a fill: X of the k-step that the sources point at into stage x, Y of the one before into y.
+    auto fill_piece = [&](int j, unsigned x, unsigned y, unsigned xmask, unsigned ymask) {
+        if (j < T::AI) {
+            const bool late = a_y[j];
+            mx_glds16(lds_base + (late ? y : x) * T::STAGE + a_dst[j], a_src + a_add[j], a_off[j], late ? ymask : xmask);
+        } else if (j < T::AI + T::WI) {
+            const int i = j - T::AI;
+            mx_glds16(lds_base + x * T::STAGE + T::A_BYTES + (i * T::NW + wave) * 1024, w_src, w_off[i], xmask);
+        } else {
+            const int i = j - T::AI - T::WI;
+            mx_glds4(lds_base + (s_y[i] ? y : x) * T::STAGE + s_dst[i], s_src[i], s_off[i], s_y[i] ? ymask : xmask);
+        }
+    };
+    auto fill_done = [&]() {
+#pragma unroll
+        for (int i = 0; i < T::SI; ++i) s_src[i] += s_step[i];
+        a_src += a_step;
+        w_src += 4096;
+    };
+
+    f32x4 acc[T::MF][4];
+#pragma unroll
+    for (int mi = 0; mi < T::MF; ++mi)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) acc[mi][f] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+    // the ring before the first k-step: X 0, then Y s and X s + 1 in pairs
+#pragma unroll
+    for (int i = 0; i < ST; ++i) {
+#pragma unroll
+        for (int j = 0; j < T::PER; ++j) fill_piece(j, i, i > 0 ? i - 1 : 0, i < nk ? ~0u : 0u, i > 0 && i - 1 < nk ? ~0u : 0u);
+        fill_done();
+    }
+    const int arow = wm * T::MF * 16 + row;
+    const int a_at = arow * 64 + (q ^ ((row >> 1) & 3)) * 16;
+    const int w_at = T::A_BYTES + wn * 4096 + lane * 16;
+    const int as_at = T::A_BYTES + T::W_BYTES + (wm * T::HR + row) * 4 + q, ws_at = T::A_BYTES + T::W_BYTES + T::AS_BYTES + wn * 256 + lane * 4;
+    // Two k-steps overlap.  The MF x 4 matrix instructions of a k-step go in MF slots of four, with the other instructions
+    // spread between the slots: slot mi reads the activations of slot mi + AHEAD; from slot TURN on, behind the barrier that
+    // publishes Y of this k-step and X of the next, the slots also issue the next fill and read the weights and first
+    // activations of k-step s + 1.  So the matrix pipe waits neither for a burst of loads nor for LDS behind the barrier.
+    constexpr int AHEAD = 1, TURN = T::HALF - AHEAD, SLOTS = T::MF - TURN;
+    struct Act { uint4 a, b; int s; };
+    struct Step { uint4 w[4]; int ws; Act x[AHEAD]; };
+    auto read_act = [&](const unsigned char* st, int mi) {
+        Act x;
+        x.a = *reinterpret_cast<const uint4*>(st + a_at + mi * 1024);
+        if constexpr (FMT == SDMI_MX_FP8) x.b = *reinterpret_cast<const uint4*>(st + a_at + BM * 64 + mi * 1024);
+        x.s = st[as_at + mi % T::HALF * 64 + mi / T::HALF * T::XJ * 256];
+        return x;
+    };
+    unsigned cur = 0, prev = ST - 1;
+    auto step = [&](auto more, const Step& c, Step& n, int s) {                  // more: k-step s + 1 exists
+        constexpr bool MORE = decltype(more)::value;
+        const unsigned char* const st = smem + cur * T::STAGE;
+        const unsigned next = cur + 1 == ST ? 0 : cur + 1;
+        const unsigned char* const nst = smem + next * T::STAGE;
+        const unsigned xmask = s + ST < nk ? ~0u : 0u, ymask = s + ST - 1 < nk ? ~0u : 0u;
+        Act x[T::MF];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) x[i] = c.x[i];
+#pragma unroll
+        for (int mi = 0; mi < T::MF; ++mi) {
+            if (mi == TURN) {
+                mx_wait<(ST - 2) * T::PER>();
+                asm volatile("s_barrier" ::: "memory");
+            }
+            if (mi + AHEAD < T::MF) x[mi + AHEAD] = read_act(st, mi + AHEAD);
+            if (mi >= TURN && MORE) {
+                const int k = mi - TURN;
+#pragma unroll
+                for (int f = 0; f < 4; ++f)
+                    if (f >= k * 4 / SLOTS && f < (k + 1) * 4 / SLOTS) n.w[f] = *reinterpret_cast<const uint4*>(nst + w_at + f * 1024);
+                if (mi == T::MF - 1) n.ws = *reinterpret_cast<const int*>(nst + ws_at);
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i)
+                    if (mi + AHEAD - i == T::MF) n.x[i] = read_act(nst, i);
+#pragma unroll
+                for (int j = 0; j < T::PER; ++j)
+                    if (j >= k * T::PER / SLOTS && j < (k + 1) * T::PER / SLOTS) fill_piece(j, cur, prev, xmask, ymask);
+            }
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+                if constexpr (FMT == SDMI_MX_FP8) acc[mi][f] = mx_mfma_f<FMT>(f, mx_op4(c.w[f]), mx_op8(x[mi].a, x[mi].b), acc[mi][f], c.ws, x[mi].s);
+                else acc[mi][f] = mx_mfma_f<FMT>(f, mx_op4(c.w[f]), mx_op4(x[mi].a), acc[mi][f], c.ws, x[mi].s);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (MORE) {
+            fill_done();
+            prev = cur;
+            cur = next;
+        }
+    };
+    Step even, odd;
+    mx_wait<(ST - 1) * T::PER>();
+    asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+    for (int f = 0; f < 4; ++f) even.w[f] = *reinterpret_cast<const uint4*>(smem + w_at + f * 1024);
+    even.ws = *reinterpret_cast<const int*>(smem + ws_at);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) even.x[i] = read_act(smem, i);
+    // Two k-steps a trip, so that the fragments of one and of the next change places without moves; an odd number is evened out
+    // in front.  One loop with one exit: with several the compiler no longer accumulates in place and spills.
+    int s = 0;
+    if ((nk - 1) & 1) {
+        step(std::true_type(), even, odd, 0);
+        even = odd;
+        s = 1;
+    }
+    for (; s + 1 < nk; s += 2) {
+        step(std::true_type(), even, odd, s);
+        step(std::true_type(), odd, even, s + 1);
+    }
+    step(std::false_type(), even, odd, s);
+
+    const int64_t n = (g0 + wn) * 64 + 16 * q;
+    if (n >= p.N) return;
+#pragma unroll
+    for (int mi = 0; mi < T::MF; ++mi) mx_store_run(p, m0 + arow + mi * 16, n, acc[mi]);
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------
@@ -170,23 +529,89 @@ static bool mx_args_ok(const sdmi_mx_gemm_args* a) {
     return !a->x || (mx_src_type(a->x_dtype) >= 0 && a->ldx >= a->K);
 }
 
+// Which kernel runs a product: the cheapest by a model of rounds.  A kernel's workgroups take `rows` x `cols` of the output; a
+// launch costs `fixed` us, a unit of K `first` for the first workgroup on each of the 256 CUs and `more` for every further
+// round of them.  (Direct kernels: the unit is eight k-steps, one for each wave; tiled ones: one k-step.)  Least squares over a
+// sweep of 1 ... 4096 rows and (N, K) of 640 x 640, 1280 x 1280, 5120 x 1280, 1280 x 5120, 5120 x 5120 and 10240 x 2560, every
+// kernel at every size; the kernel it picks is the fastest measured one, or within 14 % of it.  Examples in us, 8-bit activations:
+//     48 x  5120 x 5120: direct 16 x 64  7.2, direct 48 x 32  8.7, direct 16 x 32  8.7, tiled 64 x 128 15.2
+//    256 x  1280 x 1280: direct 48 x 32  5.0, tiled 64 x 128  6.6, tiled 128 x 128  8.8
+//    512 x  5120 x 1280: tiled 64 x 128  9.3, tiled 128 x 128  9.5, tiled 256 x 256 18.3, direct 64 x 32 23.4
+//   4096 x  5120 x 5120: tiled 128 x 128 86.9, tiled 256 x 256 102.6 (320 tiles: two rounds), tiled 64 x 128 105.7
+//   8192 x  8192 x 8192: tiled 256 x 256  366, tiled 128 x 128  439
+// Parts of K in several workgroups of a tiled kernel and a second launch that joins them were measured too (two and four parts)
+// and won by 6 % at most, at one size: the workgroups of a direct kernel split K among their waves already.
+enum MxKind { MX_D16x32, MX_D16x64, MX_D48x32, MX_D64x32, MX_T64x128, MX_T128x128, MX_T256x256, MX_KINDS };
+struct MxCost { int rows, cols, unit; struct { float fixed, first, more; } us[2]; };      // [0]: 8-bit activations, [1]: 4-bit
+static const MxCost MX_COST[MX_KINDS] = {
+    {16, 32, 8, {{2.76f, 0.482f, 0.591f}, {2.68f, 0.405f, 0.518f}}},    {16, 64, 8, {{2.69f, 0.717f, 0.983f}, {2.78f, 0.570f, 0.899f}}},
+    {48, 32, 8, {{2.96f, 0.835f, 1.476f}, {2.97f, 0.579f, 1.127f}}},    {64, 32, 8, {{2.97f, 1.072f, 1.908f}, {3.11f, 0.691f, 1.431f}}},
+    {64, 128, 1, {{3.84f, 0.278f, 0.276f}, {3.80f, 0.270f, 0.204f}}},   {128, 128, 1, {{4.37f, 0.410f, 0.432f}, {4.28f, 0.321f, 0.322f}}},
+    {256, 256, 1, {{7.88f, 1.021f, 1.603f}, {7.99f, 0.638f, 1.196f}}},
+};
+static MxKind mx_kind(const sdmi_mx_gemm_args* a) {
+    const int b = a->fmt == SDMI_MX_FP8 ? 0 : 1;
+    int best = MX_T256x256;
+    double least = 0;
+    for (int i = MX_KINDS - 1; i >= 0; --i) {
+        const MxCost& c = MX_COST[i];
+        const int64_t blocks = (a->M + c.rows - 1) / c.rows * ((a->N + c.cols - 1) / c.cols), rounds = (blocks + 255) / 256;
+        const double cost = c.us[b].fixed + (double)((mx_ksteps(a->K) + c.unit - 1) / c.unit) * (c.us[b].first + (rounds - 1) * (double)c.us[b].more);
+        if (c.unit > 1 && a->M > 65535 * (int64_t)c.rows) continue;      // the direct kernels' grid
+        if (i == MX_KINDS - 1 || cost < least) { best = i; least = cost; }
+    }
+    return (MxKind)best;
+}
+
+// The direct kernel quantises plain activations itself: one launch for up to MX_FUSED_ROWS rows whose codes fit its LDS.
+// 1 x 10240 x 5120: 8.8 us against 2.5 for the quantisation and 8.5 (4 rows x 5120 x 2560: 4.7 against 9.1); every workgroup
+// quantises all of the rows, so that it does not pay for many of them.
+static bool mx_fused(const sdmi_mx_gemm_args* a) {
+    return a->x && a->M <= MX_FUSED_ROWS && a->M * mx_ksteps(a->K) * (mx_row_bytes(128, a->fmt) + 4) <= 48 * 1024;
+}
+
 extern "C" int64_t sdmi_mx_gemm_workspace_bytes(const sdmi_mx_gemm_args* a) {
     if (!mx_args_ok(a)) return -1;
-    if (!a->x || a->M == 0) return 0;
+    if (!a->x || a->M == 0 || mx_fused(a)) return 0;
     return up256(a->M * mx_row_bytes(a->K, a->fmt)) + up256(a->M * mx_ksteps(a->K) * 4);
 }
 
-template <int FMT> static int mx_launch(const MxGemmDev& d, hipStream_t st) {
-    const unsigned nx = (unsigned)((d.N + 63) / 64 * 4);
-    const int mt = d.M <= 16 ? 1 : d.M <= 32 ? 2 : 4;
-    const int64_t ny = (d.M + 16 * mt - 1) / (16 * mt);
-    if (ny > 65535) return SDMI_ERR_BAD_ARG;
-    const dim3 g(nx, (unsigned)ny);
-    if (mt == 1) sdmi_mx_direct_kernel<FMT, 1><<<g, 256, 0, st>>>(d);
-    else if (mt == 2) sdmi_mx_direct_kernel<FMT, 2><<<g, 256, 0, st>>>(d);
-    else sdmi_mx_direct_kernel<FMT, 4><<<g, 256, 0, st>>>(d);
+template <int FMT, int BM, int WGM, int WGN, int ST> static int tiled_launch(const MxGemmDev& d, hipStream_t st) {
+    typedef MxTile<FMT, BM, WGM, WGN, ST> T;
+    static SdmiPerDeviceOnce once;
+    const auto kernel = sdmi_mx_tiled_kernel<FMT, BM, WGM, WGN, ST>;
+    if (T::LDS > 65536) {
+        const int r = once.run([&] { return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS) == hipSuccess; });
+        if (r != SDMI_OK) return r;
+    }
+    const int64_t tiles = (d.M + BM - 1) / BM * ((d.N + T::BN - 1) / T::BN);
+    if (tiles >= ((int64_t)1 << 31)) return SDMI_ERR_BAD_ARG;
+    kernel<<<(unsigned)tiles, T::THREADS, T::LDS, st>>>(d);
     SDMI_CHECK_LAUNCH();
     return SDMI_OK;
+}
+
+template <int FMT, int MT, int NF, int KW, int U, int SRC> static int direct_launch(const MxGemmDev& d, hipStream_t st) {
+    const int sums = KW * MT * NF * 1024, codes = SRC < 0 ? 0 : (int)(d.ksteps * d.M * (mx_row_bytes(128, FMT) + 4));
+    const int64_t nx = (d.N + 63) / 64 * (4 / NF), ny = (d.M + 16 * MT - 1) / (16 * MT);
+    if (ny > 65535) return SDMI_ERR_BAD_ARG;
+    sdmi_mx_direct_kernel<FMT, MT, NF, KW, U, SRC><<<dim3((unsigned)nx, (unsigned)ny), 64 * KW, sums > codes ? sums : codes, st>>>(d);
+    SDMI_CHECK_LAUNCH();
+    return SDMI_OK;
+}
+
+template <int FMT> static int mx_launch(const MxGemmDev& d, MxKind kind, int src, hipStream_t st) {
+    constexpr int ST = FMT == SDMI_MX_FP8 ? 3 : 4;
+    if (src >= 0) return src == 0 ? direct_launch<FMT, 1, 2, 8, 2, 0>(d, st) : src == 1 ? direct_launch<FMT, 1, 2, 8, 2, 1>(d, st) : direct_launch<FMT, 1, 2, 8, 2, 2>(d, st);
+    switch (kind) {
+        case MX_D16x32: return direct_launch<FMT, 1, 2, 8, 2, -1>(d, st);
+        case MX_D16x64: return direct_launch<FMT, 1, 4, 8, 2, -1>(d, st);
+        case MX_D48x32: return direct_launch<FMT, 3, 2, 8, 1, -1>(d, st);
+        case MX_D64x32: return direct_launch<FMT, 4, 2, 8, 1, -1>(d, st);
+        case MX_T64x128: return tiled_launch<FMT, 64, 2, 2, 4>(d, st);
+        case MX_T128x128: return tiled_launch<FMT, 128, 2, 2, ST>(d, st);
+        default: return tiled_launch<FMT, 256, 2, 4, ST>(d, st);
+    }
 }
 
 extern "C" int sdmi_mx_gemm(const sdmi_mx_gemm_args* a, void* stream) {
@@ -195,11 +620,16 @@ extern "C" int sdmi_mx_gemm(const sdmi_mx_gemm_args* a, void* stream) {
     if (type < 0 || a->ld_out < a->N || (a->res && a->ld_res < a->N)) return SDMI_ERR_BAD_ARG;
     if (!aligned16(a->w_codes) || !aligned16(a->w_scales) || (!a->x && (!aligned16(a->x_codes) || !aligned16(a->x_scales)))) return SDMI_ERR_ALIGNMENT;
     if (a->M == 0) return SDMI_OK;
+    const int64_t need = sdmi_mx_gemm_workspace_bytes(a);
+    if (need > 0 && (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace))) return SDMI_ERR_WORKSPACE;
     MxGemmDev d = {};
     d.xc = (const unsigned char*)a->x_codes; d.xs = (const unsigned char*)a->x_scales;
-    if (a->x) {
-        const int64_t need = sdmi_mx_gemm_workspace_bytes(a);
-        if (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace)) return SDMI_ERR_WORKSPACE;
+    int src = -1;
+    if (mx_fused(a)) {
+        src = mx_src_type(a->x_dtype);
+        d.x = a->x; d.ldx = a->ldx;
+        d.vec_x = aligned16(a->x) && a->ldx % (src == 2 ? 4 : 8) == 0;
+    } else if (a->x) {
         unsigned char* const ws = (unsigned char*)a->workspace;
         unsigned char* const xs = ws + up256(a->M * mx_row_bytes(a->K, a->fmt));
         const int st = sdmi_mx_quantize(a->x, a->ldx, a->M, a->K, a->x_dtype, ws, xs, a->fmt, stream);
@@ -208,7 +638,9 @@ extern "C" int sdmi_mx_gemm(const sdmi_mx_gemm_args* a, void* stream) {
     }
     d.wc = (const unsigned char*)a->w_codes; d.ws = (const unsigned char*)a->w_scales;
     d.bias = a->bias; d.res = a->res; d.out = a->out;
-    d.M = a->M; d.N = a->N; d.ksteps = mx_ksteps(a->K); d.ld_res = a->ld_res; d.ld_out = a->ld_out;
+    d.M = a->M; d.N = a->N; d.K = a->K; d.ksteps = mx_ksteps(a->K); d.ld_res = a->ld_res; d.ld_out = a->ld_out;
     d.type = type;
-    return a->fmt == SDMI_MX_FP8 ? mx_launch<SDMI_MX_FP8>(d, (hipStream_t)stream) : mx_launch<SDMI_MX_FP4>(d, (hipStream_t)stream);
+    d.vec_out = aligned16(a->out) && a->ld_out % (type == 2 ? 4 : 8) == 0 && aligned16(a->bias) &&
+                (!a->res || (aligned16(a->res) && a->ld_res % (type == 2 ? 4 : 8) == 0));
+    return a->fmt == SDMI_MX_FP8 ? mx_launch<SDMI_MX_FP8>(d, mx_kind(a), src, (hipStream_t)stream) : mx_launch<SDMI_MX_FP4>(d, mx_kind(a), src, (hipStream_t)stream);
 }

@@ -827,7 +827,7 @@ _MX_DT = {BF16: hip.DTYPE_BF16, F16: hip.DTYPE_F16, torch.float32: hip.DTYPE_F32
 
 class MxTensor:
     """A matrix in block-scaled form: `shape` [..., K], `fmt` "mxfp8" (e4m3) or "mxfp4" (e2m1), and on the device the codes
-    and scales that include/sdmi.h lays out - `codes` uint8 [rows, bytes of a row], `scales` uint8 [ceil(K / 128), rows, 4].
+    and scales that include/sdmi.h lays out - `codes` uint8 [planes, rows, 64] (a plane is 64 columns of mxfp8, 128 of mxfp4), `scales` uint8 [ceil(K / 128), rows, 4].
     Made by mx_quantize, rmsnorm and gated; read by linear_mx and mx_dequantize."""
     __slots__ = ("codes", "scales", "fmt", "shape")
 
@@ -917,7 +917,7 @@ class _on:
 
 def _mx_empty(rows, k, fmt, shape, device):
     steps = (k + 127) // 128
-    return MxTensor(torch.empty(rows, steps * (128 if fmt == "mxfp8" else 64), dtype=torch.uint8, device=device),
+    return MxTensor(torch.empty(steps * 2 if fmt == "mxfp8" else steps, rows, 64, dtype=torch.uint8, device=device),
                     torch.empty(steps, rows, 4, dtype=torch.uint8, device=device), fmt, shape)
 
 
@@ -937,7 +937,7 @@ def mx_quantize(x, fmt="mxfp8"):
 def mx_dequantize(q, dtype=torch.float32):
     """The values that an MxTensor stands for.  bf16 and fp32 hold them exactly (bf16 down to its subnormals); fp16 rounds."""
     dt = _mx_dt(dtype, "mx_dequantize")
-    rows, k = q.codes.shape[0], q.shape[-1]
+    rows, k = q.codes.shape[1], q.shape[-1]
     out = torch.empty(q.shape, dtype=dtype, device=q.device)
     if rows:
         with _on(out) as st:
@@ -1050,7 +1050,7 @@ def linear_mx(x, pw, fmt=None, res=None, out_dtype=None):
     if isinstance(x, MxTensor):
         if fmt is not None and fmt != x.fmt:
             raise hip.SdmiError(f"linear_mx: x is {x.fmt} already, fmt={fmt!r} was asked for")
-        m, k, ldx, x_dt, code = x.codes.shape[0], x.shape[-1], x.shape[-1], -1, _MX_FMT[x.fmt]
+        m, k, ldx, x_dt, code = x.codes.shape[1], x.shape[-1], x.shape[-1], -1, _MX_FMT[x.fmt]
         a.x_codes, a.x_scales = x.codes.data_ptr(), x.scales.data_ptr()
         out_dtype = out_dtype or (res.dtype if res is not None else BF16)
     else:
