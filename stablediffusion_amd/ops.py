@@ -827,24 +827,42 @@ _MX_DT = {BF16: hip.DTYPE_BF16, F16: hip.DTYPE_F16, torch.float32: hip.DTYPE_F32
 
 class MxTensor:
     """A matrix in block-scaled form: `shape` [..., K], `fmt` "mxfp8" (e4m3) or "mxfp4" (e2m1), and on the device the codes
-    and scales that include/sdmi.h lays out - `codes` uint8 [planes, rows, 64] (a plane is 64 columns of mxfp8, 128 of mxfp4), `scales` uint8 [ceil(K / 128), rows, 4].
-    Made by mx_quantize, rmsnorm and gated; read by linear_mx and mx_dequantize."""
-    __slots__ = ("codes", "scales", "fmt", "shape")
+    and scales that include/sdmi.h lays out - `codes` uint8 [planes, rows, 64] (a plane is 64 columns of mxfp8, 128 of mxfp4),
+    `scales` uint8 [ceil(K / 128), rows, 4].  Made by mx_quantize, rmsnorm and gated; read by linear_mx and mx_dequantize."""
+    __slots__ = ("buf", "rows", "fmt", "shape", "codes_ptr", "scales_ptr")
 
-    def __init__(self, codes, scales, fmt, shape):
-        self.codes, self.scales, self.fmt, self.shape = codes, scales, fmt, shape
+    def __init__(self, rows, fmt, shape, device):
+        # one allocation: the codes, then the scales (both multiples of 4 bytes; the scales start on 16)
+        steps = (shape[-1] + 127) // 128
+        codes = steps * rows * (128 if fmt == "mxfp8" else 64)
+        self.buf = torch.empty(codes + steps * rows * 4, dtype=torch.uint8, device=device)
+        self.rows, self.fmt, self.shape = rows, fmt, shape
+        self.codes_ptr = self.buf.data_ptr()
+        self.scales_ptr = self.codes_ptr + codes
+
+    @property
+    def codes(self):
+        steps = (self.shape[-1] + 127) // 128 * (2 if self.fmt == "mxfp8" else 1)
+        return self.buf[:steps * self.rows * 64].view(steps, self.rows, 64)
+
+    @property
+    def scales(self):
+        steps = (self.shape[-1] + 127) // 128
+        return self.buf[self.buf.numel() - steps * self.rows * 4:].view(steps, self.rows, 4)
 
     @property
     def device(self):
-        return self.codes.device
+        return self.buf.device
 
 
 class PackedMxWeight:
     """[N, K] linear weights in 4 bits with one scale per 32 (sdmi_mx_pack_linear), and the fp32 bias or None."""
-    __slots__ = ("codes", "scales", "bias", "n_out", "k")
+    __slots__ = ("codes", "scales", "bias", "n_out", "k", "codes_ptr", "scales_ptr", "bias_ptr")
 
     def __init__(self, codes, scales, bias, n_out, k):
         self.codes, self.scales, self.bias, self.n_out, self.k = codes, scales, bias, n_out, k
+        self.codes_ptr, self.scales_ptr = codes.data_ptr(), scales.data_ptr()
+        self.bias_ptr = None if bias is None else bias.data_ptr()
 
 
 def _mx_fmt(fmt):
@@ -866,59 +884,50 @@ def _mx_rows(t, name):
     column slice of a wider buffer is taken as it is."""
     if not t.is_cuda:
         raise hip.SdmiError(f"{name}: the HIP path needs device tensors (got {t.device}); there is no CPU fallback")
-    if t.dim() == 0 or t.shape[-1] == 0:
-        raise hip.SdmiError(f"{name}: needs a last axis of at least one value, got shape {tuple(t.shape)}")
-    k = t.shape[-1]
+    shape = t.shape
+    if not shape or shape[-1] == 0:
+        raise hip.SdmiError(f"{name}: needs a last axis of at least one value, got shape {tuple(shape)}")
+    k = shape[-1]
     if t.is_contiguous():
         return t.numel() // k, k, k
     if t.numel() == 0:
         return 0, k, k
-    if t.stride(-1) != 1 and k > 1:
-        raise hip.SdmiError(f"{name}: the last axis must have unit stride, got {t.stride()}")
+    strides = t.stride()
+    if strides[-1] != 1 and k > 1:
+        raise hip.SdmiError(f"{name}: the last axis must have unit stride, got {strides}")
     ld = None
     rows = 1
-    for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+    for n, s in zip(reversed(shape[:-1]), reversed(strides[:-1])):
         if n == 1:
             continue
         if ld is None:
             ld = s
         elif s != ld * rows:
-            raise hip.SdmiError(f"{name}: rows are not one stride apart (shape {tuple(t.shape)}, strides {t.stride()})")
+            raise hip.SdmiError(f"{name}: rows are not one stride apart (shape {tuple(shape)}, strides {strides})")
         rows *= n
     ld = k if ld is None else ld
     if ld < k:
-        raise hip.SdmiError(f"{name}: rows overlap (strides {t.stride()})")
+        raise hip.SdmiError(f"{name}: rows overlap (strides {strides})")
     return rows, k, ld
 
 
-def _mx_same(dev, **tensors):
+def _mx_same(device, **tensors):
     for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise hip.SdmiError(f"{name} is on {t.device}, the input on {dev}")
+        if t is not None and t.device != device:
+            raise hip.SdmiError(f"{name} is on {t.device}, the input on {device}")
 
 
-class _on:
-    """The device of a tensor made current for a launch, and its current stream."""
-    __slots__ = ("index", "before")
-
-    def __init__(self, t):
-        self.index = t.device.index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return _stream()
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
-
-
-def _mx_empty(rows, k, fmt, shape, device):
-    steps = (k + 127) // 128
-    return MxTensor(torch.empty(steps * 2 if fmt == "mxfp8" else steps, rows, 64, dtype=torch.uint8, device=device),
-                    torch.empty(steps, rows, 4, dtype=torch.uint8, device=device), fmt, shape)
+def _mx_call(fn, what, device, *args):
+    """fn(*args, stream) on `device` and its current stream.  Operators of a few microseconds: the raw handle is asked for
+    where torch.cuda.current_stream() would make an object first (0.1 us for 2.8)."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if st != hip.SDMI_OK:
+        hip.check(st, what)
 
 
 def mx_quantize(x, fmt="mxfp8"):
@@ -926,23 +935,20 @@ def mx_quantize(x, fmt="mxfp8"):
     power-of-two scale each (OCP Microscaling v1.0; a block with a NaN or an infinity becomes NaN)."""
     code, dt = _mx_fmt(fmt), _mx_dt(x.dtype, "mx_quantize")
     rows, k, ld = _mx_rows(x, "x")
-    q = _mx_empty(rows, k, fmt, x.shape, x.device)
+    q = MxTensor(rows, fmt, x.shape, x.device)
     if rows:
-        with _on(x) as st:
-            hip.check(hip.lib().sdmi_mx_quantize(x.data_ptr(), ld, rows, k, dt, q.codes.data_ptr(), q.scales.data_ptr(), code, st),
-                      "sdmi_mx_quantize")
+        _mx_call(hip.lib().sdmi_mx_quantize, "sdmi_mx_quantize", x.device, x.data_ptr(), ld, rows, k, dt, q.codes_ptr, q.scales_ptr, code)
     return q
 
 
 def mx_dequantize(q, dtype=torch.float32):
     """The values that an MxTensor stands for.  bf16 and fp32 hold them exactly (bf16 down to its subnormals); fp16 rounds."""
     dt = _mx_dt(dtype, "mx_dequantize")
-    rows, k = q.codes.shape[1], q.shape[-1]
-    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    rows, k, device = q.rows, q.shape[-1], q.buf.device
+    out = torch.empty(q.shape, dtype=dtype, device=device)
     if rows:
-        with _on(out) as st:
-            hip.check(hip.lib().sdmi_mx_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), rows, k, _MX_FMT[q.fmt], out.data_ptr(),
-                                                   k, dt, st), "sdmi_mx_dequantize")
+        _mx_call(hip.lib().sdmi_mx_dequantize, "sdmi_mx_dequantize", device, q.codes_ptr, q.scales_ptr, rows, k, _MX_FMT[q.fmt],
+                 out.data_ptr(), k, dt)
     return out
 
 
@@ -973,13 +979,11 @@ def rmsnorm(x, gamma, eps=1e-6, res=None, fmt=None, out_dtype=None):
         if out_dtype is not None:
             raise hip.SdmiError("rmsnorm: out_dtype goes with fmt=None")
         code, odt = _mx_fmt(fmt), 0
-        y = _mx_empty(rows, c, fmt, x.shape, x.device)
-        out, scales = y.codes.data_ptr(), y.scales.data_ptr()
+        y = MxTensor(rows, fmt, x.shape, x.device)
+        out, scales = y.codes_ptr, y.scales_ptr
     if rows:
-        with _on(x) as st:
-            hip.check(hip.lib().sdmi_rmsnorm(x.data_ptr(), ld, None if res is None else res.data_ptr(), ld_res, gamma.data_ptr(), eps,
-                                             rows, c, dt, None if s is None else s.data_ptr(), out, odt, scales, code, st),
-                      "sdmi_rmsnorm")
+        _mx_call(hip.lib().sdmi_rmsnorm, "sdmi_rmsnorm", x.device, x.data_ptr(), ld, None if res is None else res.data_ptr(), ld_res,
+                 gamma.data_ptr(), eps, rows, c, dt, None if s is None else s.data_ptr(), out, odt, scales, code)
     return y if res is None else (y, s)
 
 
@@ -1003,11 +1007,10 @@ def gated(x, act="gelu", fmt=None, out_dtype=None):
         if out_dtype is not None:
             raise hip.SdmiError("gated: out_dtype goes with fmt=None")
         code, odt = _mx_fmt(fmt), 0
-        y = _mx_empty(rows, c, fmt, shape, x.device)
-        out, scales = y.codes.data_ptr(), y.scales.data_ptr()
+        y = MxTensor(rows, fmt, shape, x.device)
+        out, scales = y.codes_ptr, y.scales_ptr
     if rows:
-        with _on(x) as st:
-            hip.check(hip.lib().sdmi_gated(x.data_ptr(), ld, rows, c, dt, _GATES[act], out, odt, scales, code, st), "sdmi_gated")
+        _mx_call(hip.lib().sdmi_gated, "sdmi_gated", x.device, x.data_ptr(), ld, rows, c, dt, _GATES[act], out, odt, scales, code)
     return y
 
 
@@ -1028,10 +1031,20 @@ def pack_linear_mx(weight, bias=None):
     lib = hip.lib()
     pw = PackedMxWeight(torch.empty(lib.sdmi_mx_weight_codes_bytes(n, k), dtype=torch.uint8, device=w.device),
                         torch.empty(lib.sdmi_mx_weight_scales_bytes(n, k), dtype=torch.uint8, device=w.device), b, n, k)
-    with _on(w) as st:
-        hip.check(lib.sdmi_mx_pack_linear(w.data_ptr(), ld, n, k, dt, pw.codes.data_ptr(), pw.scales.data_ptr(), st),
-                  "sdmi_mx_pack_linear")
+    _mx_call(lib.sdmi_mx_pack_linear, "sdmi_mx_pack_linear", w.device, w.data_ptr(), ld, n, k, dt, pw.codes.data_ptr(), pw.scales.data_ptr())
     return pw
+
+
+def _mx_scratch(nbytes, device):
+    """_scratch() for `device`, which need not be the current one."""
+    index = device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _scratch(nbytes, device)
+    buf = _SCRATCH.get((index, torch._C._cuda_getCurrentRawStream(index)))
+    if buf is not None and buf.numel() >= nbytes and not torch.cuda.is_current_stream_capturing():
+        return buf
+    return _scratch(nbytes, device)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1050,37 +1063,34 @@ def linear_mx(x, pw, fmt=None, res=None, out_dtype=None):
     if isinstance(x, MxTensor):
         if fmt is not None and fmt != x.fmt:
             raise hip.SdmiError(f"linear_mx: x is {x.fmt} already, fmt={fmt!r} was asked for")
-        m, k, ldx, x_dt, code = x.codes.shape[1], x.shape[-1], x.shape[-1], -1, _MX_FMT[x.fmt]
-        a.x_codes, a.x_scales = x.codes.data_ptr(), x.scales.data_ptr()
+        m, k, ldx, x_dt, code, dev = x.rows, x.shape[-1], 0, -1, _MX_FMT[x.fmt], x.buf.device
+        a.x_codes, a.x_scales = x.codes_ptr, x.scales_ptr
         out_dtype = out_dtype or (res.dtype if res is not None else BF16)
     else:
-        code, x_dt = _mx_fmt(fmt or "mxfp8"), _mx_dt(x.dtype, "linear_mx")
+        code, x_dt, dev = _mx_fmt(fmt or "mxfp8"), _mx_dt(x.dtype, "linear_mx"), x.device
         m, k, ldx = _mx_rows(x, "x")
         a.x, a.ldx, a.x_dtype = x.data_ptr(), ldx, x_dt
         out_dtype = out_dtype or x.dtype
     if k != pw.k:
         raise hip.SdmiError(f"linear_mx: K mismatch ({k} vs packed {pw.k})")
-    dev, n = x.device, pw.n_out
-    shape = torch.Size((*x.shape[:-1], n))
+    n = pw.n_out
+    shape = (*x.shape[:-1], n)
     _mx_same(dev, weight=pw.codes, res=res)
     a.out_dtype = _mx_dt(out_dtype, "linear_mx out_dtype")
     if res is not None:
         if res.dtype != out_dtype or res.shape != shape:
-            raise hip.SdmiError(f"linear_mx: res is {res.dtype} {tuple(res.shape)}, the output {out_dtype} {tuple(shape)}")
+            raise hip.SdmiError(f"linear_mx: res is {res.dtype} {tuple(res.shape)}, the output {out_dtype} {shape}")
         a.res, a.ld_res = res.data_ptr(), _mx_rows(res, "res")[2]
     out = torch.empty(shape, dtype=out_dtype, device=dev)
     if m == 0:
         return out
     a.M, a.N, a.K, a.fmt, a.ld_out = m, n, k, code, n
-    a.w_codes, a.w_scales, a.out = pw.codes.data_ptr(), pw.scales.data_ptr(), out.data_ptr()
-    if pw.bias is not None:
-        a.bias = pw.bias.data_ptr()
-    with _on(out) as st:
-        nbytes = _mx_gemm_workspace(m, n, k, ldx, x_dt, code)
-        if nbytes > 0:
-            ws = _scratch(nbytes, dev)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-        hip.check(hip.lib().sdmi_mx_gemm(C.byref(a), st), "sdmi_mx_gemm")
+    a.w_codes, a.w_scales, a.out, a.bias = pw.codes_ptr, pw.scales_ptr, out.data_ptr(), pw.bias_ptr
+    nbytes = _mx_gemm_workspace(m, n, k, ldx, x_dt, code)
+    if nbytes > 0:
+        ws = _mx_scratch(nbytes, dev)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    _mx_call(hip.lib().sdmi_mx_gemm, "sdmi_mx_gemm", dev, C.byref(a))
     return out
 
 
