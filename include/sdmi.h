@@ -425,8 +425,8 @@ int sdmi_image_to_u8(const float* x, uint8_t* out, int32_t nb, int32_t C, int64_
  *       sdmi_mx_scales_bytes (-1 for sizes that are refused).
  *   weights: an opaque order of the same values (sdmi_mx_pack_linear).
  * dtype / out_dtype: SDMI_DTYPE_BF16 | _F16 | _F32.  Leading dimensions count elements; rows may be strided, the inner
- * stride is 1.  16-byte aligned rows (pointer, and leading dimension a multiple of 8, or 4 for fp32) are read in vectors,
- * others element by element.  Codes, scales, packed weights, gamma and workspaces are 16-byte aligned (else SDMI_ERR_ALIGNMENT).
+ * stride is 1, and a row may start at any element.  Codes, scales, packed weights, gamma and workspaces are 16-byte aligned
+ * (else SDMI_ERR_ALIGNMENT).
  * rows == 0 is a valid empty call.  Outputs may not overlap inputs.
  *   sdmi_mx_quantize:   [rows, K] -> codes, scales
  *   sdmi_mx_dequantize: the values that codes and scales stand for (bf16 and fp32 hold them exactly, but for bf16's range)

@@ -28,15 +28,19 @@ template <int T> __device__ __forceinline__ float mx_to_f32(typename MxElem<T>::
     else return elem_to_f32<T>(v);
 }
 
-// 8 consecutive values from p[0..]; `n` of them exist (the others read as 0).  vec: p is aligned to a 16-byte vector.
-template <int T> __device__ __forceinline__ void mx_load8(const typename MxElem<T>::type* p, int n, bool vec, float* f) {
-    if (vec && n >= 8) {
+// 8 consecutive values from p[0..], of which `n` exist (the others read as 0).  Vector memory instructions take any address
+// that the element's own alignment allows, so rows that are not 16-byte aligned - an odd width, a column slice - are read in
+// vectors like others.
+typedef uint4 __attribute__((aligned(2))) mx_u128_a2;
+typedef f32x4 __attribute__((aligned(4))) mx_f128_a4;
+template <int T> __device__ __forceinline__ void mx_load8(const typename MxElem<T>::type* p, int n, float* f) {
+    if (n >= 8) {
         if constexpr (T == 2) {
-            const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+            const f32x4 a = reinterpret_cast<const mx_f128_a4*>(p)[0], b = reinterpret_cast<const mx_f128_a4*>(p)[1];
 #pragma unroll
             for (int j = 0; j < 4; ++j) { f[j] = a[j]; f[4 + j] = b[j]; }
         } else {
-            elem_unpack8<T>(*reinterpret_cast<const uint4*>(p), f);
+            elem_unpack8<T>(*reinterpret_cast<const mx_u128_a2*>(p), f);
         }
     } else {
 #pragma unroll
@@ -44,13 +48,13 @@ template <int T> __device__ __forceinline__ void mx_load8(const typename MxElem<
     }
 }
 // 8 consecutive values to p[0..], of which `n` exist.
-template <int T> __device__ __forceinline__ void mx_store8(typename MxElem<T>::type* p, int n, bool vec, const float* f) {
-    if (vec && n >= 8) {
+template <int T> __device__ __forceinline__ void mx_store8(typename MxElem<T>::type* p, int n, const float* f) {
+    if (n >= 8) {
         if constexpr (T == 2) {
-            reinterpret_cast<f32x4*>(p)[0] = (f32x4){f[0], f[1], f[2], f[3]};
-            reinterpret_cast<f32x4*>(p)[1] = (f32x4){f[4], f[5], f[6], f[7]};
+            reinterpret_cast<mx_f128_a4*>(p)[0] = (f32x4){f[0], f[1], f[2], f[3]};
+            reinterpret_cast<mx_f128_a4*>(p)[1] = (f32x4){f[4], f[5], f[6], f[7]};
         } else {
-            *reinterpret_cast<uint4*>(p) = elem_pack8<T>(f);
+            *reinterpret_cast<mx_u128_a2*>(p) = elem_pack8<T>(f);
         }
     } else {
 #pragma unroll
@@ -128,14 +132,13 @@ template <int FMT> __device__ __forceinline__ unsigned mx_quantise8(const float*
 // erfc(z) = exp(-z^2) t P(t), t = 1 / (1 + 0.375 z), P a degree-6 polynomial fitted to exp(z^2) erfc(z) on [0, 10]
 // (relative error 6.4e-7).  Written from the small side, so that the tail of negative x keeps its relative precision.
 __device__ __forceinline__ float mx_gelu(float x) {
-    const float z = fabsf(x) * 0.70710678118654752f;
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.375f, z, 1.0f));
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.375f * 0.70710678118654752f, fabsf(x), 1.0f));
     float p = fmaf(-1.350968426e-01f, t, 3.879412549e-01f);
     p = fmaf(p, t, -1.296022628e-01f);
     p = fmaf(p, t, 2.830651671e-01f);
     p = fmaf(p, t, 1.666631723e-01f);
     p = fmaf(p, t, 2.156894433e-01f);
     p = fmaf(p, t, 2.113394301e-01f);
-    const float half = 0.5f * p * t * __expf(-0.5f * x * x);     // Phi(-|x|); z^2 as x^2 / 2: one rounding before the exponential
+    const float half = (0.5f * p * t) * __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f);      // Phi(-|x|); exp(-z^2) = 2^(-x^2 / (2 ln 2))
     return x * (x < 0.0f ? half : 1.0f - half);
 }

@@ -5,10 +5,11 @@
 #include "sdmi_mx.h"
 
 // ---- one k-step per 16 lanes -------------------------------------------------------------------------------------------
-// A block of 256 threads owns a tile of 16 rows x 4 k-steps (512 values): 16 lanes hold one k-step of one row, 8 values a
-// lane, and walk the four k-steps.  So a row's 1 KB is read in 256-byte runs, and the 16 scale dwords of a k-step lie next
-// to each other.
-constexpr int EL_ROWS = 16, EL_STEPS = 4;
+// A block of 256 threads owns a tile of 16 rows x STEPS k-steps: 16 lanes hold one k-step of one row, 8 values a lane.  So a
+// row is read in 256-byte runs, the 16 rows of a code plane are written as one KB, and the 16 scale dwords of a k-step lie next
+// to each other.  STEPS = 4 keeps four (gated: eight) loads a lane in flight; a launch too small to fill the chip with such
+// tiles takes STEPS = 1, four times the waves with a quarter of the instructions each (gated 1 x 1280: 5.2 -> 3.2 us, 154 x 4096: 5.6 -> 3.5).
+constexpr int EL_ROWS = 16;
 
 struct MxElemArgs {
     const void* x;
@@ -18,11 +19,10 @@ struct MxElemArgs {
     unsigned char* codes;
     unsigned char* scales;
     unsigned ktiles;
-    int vec_in, vec_gate, vec_out;
 };
 
 // OP 0: x   1: a gelu(b)   2: a silu(b)        FMT -1: plain result of type TO
-template <int T, int OP, int FMT, int TO>
+template <int T, int OP, int FMT, int TO, int EL_STEPS>
 __global__ __launch_bounds__(256) void sdmi_mx_elem_kernel(MxElemArgs p) {
     typedef typename MxElem<T>::type E;
     const unsigned tile_r = blockIdx.x / p.ktiles, tile_k = blockIdx.x - tile_r * p.ktiles;
@@ -36,8 +36,8 @@ __global__ __launch_bounds__(256) void sdmi_mx_elem_kernel(MxElemArgs p) {
     for (int s = 0; s < EL_STEPS; ++s) {
         const int64_t k0 = ((int64_t)tile_k * EL_STEPS + s) * MX_KSTEP + sub * 8;
         const int n = (int)max((int64_t)0, min((int64_t)8, p.K - k0));
-        mx_load8<T>(xr + k0, n, p.vec_in, f[s]);
-        if constexpr (OP != 0) mx_load8<T>(xr + p.K + k0, n, p.vec_gate, g[s]);
+        mx_load8<T>(xr + k0, n, f[s]);
+        if constexpr (OP != 0) mx_load8<T>(xr + p.K + k0, n, g[s]);
     }
 #pragma unroll
     for (int s = 0; s < EL_STEPS; ++s) {
@@ -54,7 +54,7 @@ __global__ __launch_bounds__(256) void sdmi_mx_elem_kernel(MxElemArgs p) {
         }
         if constexpr (FMT < 0) {
             if (row < p.rows && n > 0)
-                mx_store8<TO>(reinterpret_cast<typename MxElem<TO>::type*>(p.out) + row * p.ld_out + k0, n, p.vec_out, f[s]);
+                mx_store8<TO>(reinterpret_cast<typename MxElem<TO>::type*>(p.out) + row * p.ld_out + k0, n, f[s]);
         } else {
             uint2 c;
             const unsigned dw = mx_quantise8<FMT>(f[s], lane, c);
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void sdmi_mx_elem_kernel(MxElemArgs p) {
 
 // The values that codes and scales stand for.  Every code has at most four significant bits: a bf16 holds the value exactly
 // (down to its subnormals), an f16 rounds it to its own range.
-template <int FMT, int TO>
+template <int FMT, int TO, int EL_STEPS>
 __global__ __launch_bounds__(256) void sdmi_mx_dequantise_kernel(MxElemArgs p) {
     const unsigned tile_r = blockIdx.x / p.ktiles, tile_k = blockIdx.x - tile_r * p.ktiles;
     const int sub = threadIdx.x & 15;
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(256) void sdmi_mx_dequantise_kernel(MxElemArgs p) {
         const float scale = __uint_as_float(byte == 0u ? 0x00400000u : byte == 255u ? 0x7fc00000u : byte << 23);
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] *= scale;
-        mx_store8<TO>(reinterpret_cast<typename MxElem<TO>::type*>(p.out) + row * p.ld_out + k0, n, p.vec_out, f);
+        mx_store8<TO>(reinterpret_cast<typename MxElem<TO>::type*>(p.out) + row * p.ld_out + k0, n, f);
     }
 }
 
@@ -126,7 +126,6 @@ struct MxNormArgs {
     unsigned char* scales;
     int64_t ldx, ld_res, rows, C;
     float eps;
-    int vec_x, vec_res, vec_out;
 };
 
 template <int T, int FMT, int TO, int TPR, int U>
@@ -135,14 +134,20 @@ __global__ __launch_bounds__(256) void sdmi_rmsnorm_kernel(MxNormArgs p) {
     constexpr int RPB = 256 / TPR;
     __shared__ float part[RPB][TPR / 64];
     const int t = threadIdx.x % TPR, r = threadIdx.x / TPR, lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * RPB + r, srow = row < p.rows ? row : p.rows - 1;
+    // Workgroups go round the 8 XCDs; of every 64 each XCD takes 8 neighbours, whose codes and scales share cache lines of its
+    // L2 (16384 x 5120 with residual and 8-bit output: 129 -> 120 us; runs of 2 and 32 the same or slower, one run an XCD 152:
+    // eight far places of memory at a time).
+    constexpr unsigned RUN = 8;
+    unsigned block = blockIdx.x;
+    if (block < gridDim.x / (8 * RUN) * (8 * RUN)) block = block / (8 * RUN) * (8 * RUN) + (block & 7) * RUN + block % (8 * RUN) / 8;
+    const int64_t row = (int64_t)block * RPB + r, srow = row < p.rows ? row : p.rows - 1;
     const E* const xr = reinterpret_cast<const E*>(p.x) + srow * p.ldx;
     float f[U][8], q[U][8];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int64_t c0 = ((int64_t)u * TPR + t) * 8;
         const int n = (int)max((int64_t)0, min((int64_t)8, p.C - c0));
-        mx_load8<T>(xr + c0, n, p.vec_x, f[u]);
+        mx_load8<T>(xr + c0, n, f[u]);
     }
     if (p.res) {
         const E* const rr = reinterpret_cast<const E*>(p.res) + srow * p.ld_res;
@@ -150,7 +155,7 @@ __global__ __launch_bounds__(256) void sdmi_rmsnorm_kernel(MxNormArgs p) {
         for (int u = 0; u < U; ++u) {
             const int64_t c0 = ((int64_t)u * TPR + t) * 8;
             const int n = (int)max((int64_t)0, min((int64_t)8, p.C - c0));
-            mx_load8<T>(rr + c0, n, p.vec_res, q[u]);
+            mx_load8<T>(rr + c0, n, q[u]);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -178,14 +183,14 @@ __global__ __launch_bounds__(256) void sdmi_rmsnorm_kernel(MxNormArgs p) {
         const int64_t c0 = ((int64_t)u * TPR + t) * 8;
         const int n = (int)max((int64_t)0, min((int64_t)8, p.C - c0));
         if (p.sum_out && row < p.rows && n > 0)
-            mx_store8<T>(reinterpret_cast<E*>(p.sum_out) + row * p.C + c0, n, p.vec_out, f[u]);
+            mx_store8<T>(reinterpret_cast<E*>(p.sum_out) + row * p.C + c0, n, f[u]);
         float gm[8];
-        mx_load8<2>(p.gamma + c0, n, true, gm);
+        mx_load8<2>(p.gamma + c0, n, gm);
 #pragma unroll
         for (int j = 0; j < 8; ++j) gm[j] *= f[u][j] * rstd;
         if constexpr (FMT < 0) {
             if (row < p.rows && n > 0)
-                mx_store8<TO>(reinterpret_cast<typename MxElem<TO>::type*>(p.out) + row * p.C + c0, n, p.vec_out, gm);
+                mx_store8<TO>(reinterpret_cast<typename MxElem<TO>::type*>(p.out) + row * p.C + c0, n, gm);
         } else {
             const int64_t step = c0 / MX_KSTEP;
             if (step >= nsteps) continue;                        // (whole groups of 16 lanes)
@@ -204,7 +209,6 @@ __global__ __launch_bounds__(256) void sdmi_rmsnorm_kernel(MxNormArgs p) {
 
 // ---- host side ---------------------------------------------------------------------------------------------------------
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-static bool vec_rows(const void* p, int64_t ld, int type) { return aligned16(p) && ld % (type == 2 ? 4 : 8) == 0; }
 static bool fmt_ok(int32_t fmt) { return fmt == SDMI_MX_FP8 || fmt == SDMI_MX_FP4; }
 constexpr int64_t MX_MAX_K = (int64_t)1 << 24, MX_MAX_ROWS = ((int64_t)1 << 31) - 1;
 
@@ -213,22 +217,28 @@ extern "C" int64_t sdmi_mx_codes_bytes(int64_t rows, int64_t K, int32_t fmt) {
 }
 extern "C" int64_t sdmi_mx_scales_bytes(int64_t rows, int64_t K) { return rows < 0 || K <= 0 ? -1 : rows * mx_ksteps(K) * 4; }
 
-// Whether the tiles of a launch fit a grid (grid.x < 2^31); `ktiles` is set.
-static bool elem_grid(int64_t rows, int64_t K, unsigned* ktiles, unsigned* blocks) {
-    const int64_t kt = (mx_ksteps(K) + EL_STEPS - 1) / EL_STEPS, n = (rows + EL_ROWS - 1) / EL_ROWS * kt;
-    *ktiles = (unsigned)kt;
-    *blocks = (unsigned)n;
-    return n < ((int64_t)1 << 31);
+// The tiles of a launch and the k-steps of each; false: more than a grid holds.
+struct ElemGrid { unsigned blocks; int steps; };
+static bool elem_grid(int64_t rows, int64_t K, MxElemArgs* a, ElemGrid* g) {
+    const int64_t rt = (rows + EL_ROWS - 1) / EL_ROWS, ks = mx_ksteps(K);
+    g->steps = rt * ((ks + 3) / 4) >= 1024 ? 4 : 1;
+    a->ktiles = (unsigned)((ks + g->steps - 1) / g->steps);
+    g->blocks = (unsigned)(rt * a->ktiles);
+    return rt * a->ktiles < ((int64_t)1 << 31);
 }
 
+template <int T, int OP, int FMT, int TO> static void elem_steps(const MxElemArgs& a, const ElemGrid& g, hipStream_t st) {
+    if (g.steps == 4) sdmi_mx_elem_kernel<T, OP, FMT, TO, 4><<<g.blocks, 256, 0, st>>>(a);
+    else sdmi_mx_elem_kernel<T, OP, FMT, TO, 1><<<g.blocks, 256, 0, st>>>(a);
+}
 template <int T, int OP>
-static int elem_launch(const MxElemArgs& a, int fmt, int to, unsigned blocks, hipStream_t st) {
-    if (fmt == SDMI_MX_FP8) sdmi_mx_elem_kernel<T, OP, SDMI_MX_FP8, 0><<<blocks, 256, 0, st>>>(a);
-    else if (fmt == SDMI_MX_FP4) sdmi_mx_elem_kernel<T, OP, SDMI_MX_FP4, 0><<<blocks, 256, 0, st>>>(a);
+static int elem_launch(const MxElemArgs& a, int fmt, int to, const ElemGrid& g, hipStream_t st) {
+    if (fmt == SDMI_MX_FP8) elem_steps<T, OP, SDMI_MX_FP8, 0>(a, g, st);
+    else if (fmt == SDMI_MX_FP4) elem_steps<T, OP, SDMI_MX_FP4, 0>(a, g, st);
     else if constexpr (OP == 0) return SDMI_ERR_BAD_ARG;
-    else if (to == 0) sdmi_mx_elem_kernel<T, OP, -1, 0><<<blocks, 256, 0, st>>>(a);
-    else if (to == 1) sdmi_mx_elem_kernel<T, OP, -1, 1><<<blocks, 256, 0, st>>>(a);
-    else sdmi_mx_elem_kernel<T, OP, -1, 2><<<blocks, 256, 0, st>>>(a);
+    else if (to == 0) elem_steps<T, OP, -1, 0>(a, g, st);
+    else if (to == 1) elem_steps<T, OP, -1, 1>(a, g, st);
+    else elem_steps<T, OP, -1, 2>(a, g, st);
     SDMI_CHECK_LAUNCH();
     return SDMI_OK;
 }
@@ -241,11 +251,10 @@ extern "C" int sdmi_mx_quantize(const void* x, int64_t ldx, int64_t rows, int64_
     if (rows == 0) return SDMI_OK;
     MxElemArgs a = {};
     a.x = x; a.ldx = ldx; a.rows = rows; a.K = K; a.codes = (unsigned char*)codes; a.scales = (unsigned char*)scales;
-    a.vec_in = vec_rows(x, ldx, t);
-    unsigned blocks;
-    if (!elem_grid(rows, K, &a.ktiles, &blocks)) return SDMI_ERR_BAD_ARG;
+    ElemGrid g;
+    if (!elem_grid(rows, K, &a, &g)) return SDMI_ERR_BAD_ARG;
     hipStream_t st = (hipStream_t)stream;
-    return t == 0 ? elem_launch<0, 0>(a, fmt, 0, blocks, st) : t == 1 ? elem_launch<1, 0>(a, fmt, 0, blocks, st) : elem_launch<2, 0>(a, fmt, 0, blocks, st);
+    return t == 0 ? elem_launch<0, 0>(a, fmt, 0, g, st) : t == 1 ? elem_launch<1, 0>(a, fmt, 0, g, st) : elem_launch<2, 0>(a, fmt, 0, g, st);
 }
 
 extern "C" int sdmi_gated(const void* x, int64_t ldx, int64_t rows, int64_t inner, int32_t dtype, int32_t act, void* out,
@@ -258,15 +267,12 @@ extern "C" int sdmi_gated(const void* x, int64_t ldx, int64_t rows, int64_t inne
     MxElemArgs a = {};
     a.x = x; a.ldx = ldx; a.rows = rows; a.K = inner; a.codes = (unsigned char*)out; a.scales = (unsigned char*)scales;
     a.out = out; a.ld_out = inner;
-    a.vec_in = vec_rows(x, ldx, t);
-    a.vec_gate = a.vec_in && inner % (t == 2 ? 4 : 8) == 0;
-    a.vec_out = vec_rows(out, inner, to);
-    unsigned blocks;
-    if (!elem_grid(rows, inner, &a.ktiles, &blocks)) return SDMI_ERR_BAD_ARG;
+    ElemGrid g;
+    if (!elem_grid(rows, inner, &a, &g)) return SDMI_ERR_BAD_ARG;
     hipStream_t st = (hipStream_t)stream;
     if (act == 0)
-        return t == 0 ? elem_launch<0, 1>(a, fmt, to, blocks, st) : t == 1 ? elem_launch<1, 1>(a, fmt, to, blocks, st) : elem_launch<2, 1>(a, fmt, to, blocks, st);
-    return t == 0 ? elem_launch<0, 2>(a, fmt, to, blocks, st) : t == 1 ? elem_launch<1, 2>(a, fmt, to, blocks, st) : elem_launch<2, 2>(a, fmt, to, blocks, st);
+        return t == 0 ? elem_launch<0, 1>(a, fmt, to, g, st) : t == 1 ? elem_launch<1, 1>(a, fmt, to, g, st) : elem_launch<2, 1>(a, fmt, to, g, st);
+    return t == 0 ? elem_launch<0, 2>(a, fmt, to, g, st) : t == 1 ? elem_launch<1, 2>(a, fmt, to, g, st) : elem_launch<2, 2>(a, fmt, to, g, st);
 }
 
 extern "C" int sdmi_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t K, int32_t fmt, void* out,
@@ -277,11 +283,10 @@ extern "C" int sdmi_mx_dequantize(const void* codes, const void* scales, int64_t
     if (rows == 0) return SDMI_OK;
     MxElemArgs a = {};
     a.rows = rows; a.K = K; a.codes = (unsigned char*)codes; a.scales = (unsigned char*)scales; a.out = out; a.ld_out = ld_out;
-    a.vec_out = vec_rows(out, ld_out, to);
-    unsigned blocks;
-    if (!elem_grid(rows, K, &a.ktiles, &blocks)) return SDMI_ERR_BAD_ARG;
+    ElemGrid g;
+    if (!elem_grid(rows, K, &a, &g)) return SDMI_ERR_BAD_ARG;
     hipStream_t st = (hipStream_t)stream;
-#define SDMI_DQ(F, O) sdmi_mx_dequantise_kernel<F, O><<<blocks, 256, 0, st>>>(a)
+#define SDMI_DQ(F, O) do { if (g.steps == 4) sdmi_mx_dequantise_kernel<F, O, 4><<<g.blocks, 256, 0, st>>>(a); else sdmi_mx_dequantise_kernel<F, O, 1><<<g.blocks, 256, 0, st>>>(a); } while (0)
     if (fmt == SDMI_MX_FP8) { if (to == 0) SDMI_DQ(SDMI_MX_FP8, 0); else if (to == 1) SDMI_DQ(SDMI_MX_FP8, 1); else SDMI_DQ(SDMI_MX_FP8, 2); }
     else { if (to == 0) SDMI_DQ(SDMI_MX_FP4, 0); else if (to == 1) SDMI_DQ(SDMI_MX_FP4, 1); else SDMI_DQ(SDMI_MX_FP4, 2); }
 #undef SDMI_DQ
@@ -291,14 +296,22 @@ extern "C" int sdmi_mx_dequantize(const void* codes, const void* scales, int64_t
 
 template <int T, int FMT, int TO>
 static int norm_launch(const MxNormArgs& a, hipStream_t st) {
-    // 64 threads a row up to 1024 values (four rows a block), 256 above
+    // As few threads a row as hold it in one chunk of 8 values each, and from 2048 values on 256 threads with as many chunks as
+    // the row needs and no more: an empty chunk costs registers and instructions (16384 x 5120: 256 x 3 120 us, 256 x 4 143,
+    // 128 x 5 148, 512 x 2 127, 64 x 10 208; 32768 x 1024: 128 x 1 47 us, 64 x 2 50, 256 x 1 58).
 #define SDMI_NORM(TPR, U) sdmi_rmsnorm_kernel<T, FMT, TO, TPR, U><<<(unsigned)((a.rows + 256 / TPR - 1) / (256 / TPR)), 256, 0, st>>>(a)
     if (a.C <= 512) SDMI_NORM(64, 1);
-    else if (a.C <= 1024) SDMI_NORM(64, 2);
-    else if (a.C <= 2048) SDMI_NORM(256, 1);
-    else if (a.C <= 4096) SDMI_NORM(256, 2);
-    else if (a.C <= 8192) SDMI_NORM(256, 4);
-    else SDMI_NORM(256, 8);
+    else if (a.C <= 1024) SDMI_NORM(128, 1);
+    else switch ((a.C + 2047) / 2048) {
+        case 1: SDMI_NORM(256, 1); break;
+        case 2: SDMI_NORM(256, 2); break;
+        case 3: SDMI_NORM(256, 3); break;
+        case 4: SDMI_NORM(256, 4); break;
+        case 5: SDMI_NORM(256, 5); break;
+        case 6: SDMI_NORM(256, 6); break;
+        case 7: SDMI_NORM(256, 7); break;
+        default: SDMI_NORM(256, 8);
+    }
 #undef SDMI_NORM
     SDMI_CHECK_LAUNCH();
     return SDMI_OK;
@@ -322,9 +335,6 @@ extern "C" int sdmi_rmsnorm(const void* x, int64_t ldx, const void* res, int64_t
     a.x = x; a.res = res; a.gamma = gamma; a.sum_out = res ? sum_out : nullptr; a.out = out;
     a.codes = (unsigned char*)out; a.scales = (unsigned char*)scales;
     a.ldx = ldx; a.ld_res = ld_res; a.rows = rows; a.C = C; a.eps = eps;
-    a.vec_x = vec_rows(x, ldx, t);
-    a.vec_res = res ? vec_rows(res, ld_res, t) : 0;
-    a.vec_out = C % 8 == 0 && (fmt != SDMI_MX_NONE || aligned16(out)) && (!a.sum_out || aligned16(a.sum_out));
     hipStream_t st = (hipStream_t)stream;
     return t == 0 ? norm_type<0>(a, fmt, to, st) : t == 1 ? norm_type<1>(a, fmt, to, st) : norm_type<2>(a, fmt, to, st);
 }

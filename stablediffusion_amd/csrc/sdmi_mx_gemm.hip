@@ -17,7 +17,7 @@ typedef __attribute__((ext_vector_type(8))) int i32x8;
 // ---- packing -----------------------------------------------------------------------------------------------------------
 template <int T>
 __global__ __launch_bounds__(256) void sdmi_mx_pack_kernel(const typename MxElem<T>::type* w, int64_t ldw, int64_t N, int64_t K,
-                                                           unsigned char* codes, unsigned char* scales, int vec) {
+                                                           unsigned char* codes, unsigned char* scales) {
     const int64_t ksteps = mx_ksteps(K), kblocks = ksteps * 4, np = (N + 63) / 64 * 64;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= np * kblocks) return;
@@ -28,7 +28,7 @@ __global__ __launch_bounds__(256) void sdmi_mx_pack_kernel(const typename MxElem
     for (int j = 0; j < 4; ++j) {
         const int64_t k0 = kb * 32 + j * 8;
         const int have = n < N ? (int)max((int64_t)0, min((int64_t)8, K - k0)) : 0;
-        mx_load8<T>(w + (n < N ? n : 0) * ldw + k0, have, vec, f[j]);
+        mx_load8<T>(w + (n < N ? n : 0) * ldw + k0, have, f[j]);
         m = max(m, mx_amax8(f[j]));
     }
     const unsigned byte = mx_scale_byte<SDMI_MX_FP4>(m);
@@ -56,7 +56,6 @@ struct MxGemmDev {
     void* out;
     const void* x;             // the direct form that quantises: plain activations
     int64_t M, N, K, ksteps, ldx, ld_res, ld_out;
-    int vec_x, vec_out;
     int type;                  // of out and res: 0 bf16, 1 f16, 2 fp32
 };
 
@@ -101,7 +100,7 @@ __device__ __forceinline__ void mx_store_quad(const MxGemmDev& p, int64_t m, int
 // out[m, n .. n + 16): the four quads of a lane are consecutive columns
 __device__ __forceinline__ void mx_store_run(const MxGemmDev& p, int64_t m, int64_t n, const f32x4* v) {
     if (m >= p.M) return;
-    if (!p.vec_out || n + 16 > p.N) {
+    if (n + 16 > p.N) {
 #pragma unroll
         for (int f = 0; f < 4; ++f) mx_store_quad(p, m, n + 4 * f, v[f]);
         return;
@@ -114,7 +113,7 @@ __device__ __forceinline__ void mx_store_run(const MxGemmDev& p, int64_t m, int6
     if (p.bias) {
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
-            const f32x4 b = *reinterpret_cast<const f32x4*>(p.bias + n + 4 * f);
+            const f32x4 b = *reinterpret_cast<const mx_f128_a4*>(p.bias + n + 4 * f);
 #pragma unroll
             for (int r = 0; r < 4; ++r) a[4 * f + r] += b[r];
         }
@@ -124,19 +123,19 @@ __device__ __forceinline__ void mx_store_run(const MxGemmDev& p, int64_t m, int6
         float b[8];
         if (p.type == 2) {
             if (p.res) {
-                mx_load8<2>(reinterpret_cast<const float*>(p.res) + m * p.ld_res + n + 8 * h, 8, true, b);
+                mx_load8<2>(reinterpret_cast<const float*>(p.res) + m * p.ld_res + n + 8 * h, 8, b);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) a[8 * h + j] += b[j];
             }
-            mx_store8<2>(reinterpret_cast<float*>(p.out) + m * p.ld_out + n + 8 * h, 8, true, a + 8 * h);
+            mx_store8<2>(reinterpret_cast<float*>(p.out) + m * p.ld_out + n + 8 * h, 8, a + 8 * h);
         } else {
             if (p.res) {
-                const uint4 r = *reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned short*>(p.res) + m * p.ld_res + n + 8 * h);
+                const uint4 r = *reinterpret_cast<const mx_u128_a2*>(reinterpret_cast<const unsigned short*>(p.res) + m * p.ld_res + n + 8 * h);
                 if (p.type == 0) elem_unpack8<0>(r, b); else elem_unpack8<1>(r, b);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) a[8 * h + j] += b[j];
             }
-            *reinterpret_cast<uint4*>(reinterpret_cast<unsigned short*>(p.out) + m * p.ld_out + n + 8 * h) =
+            *reinterpret_cast<mx_u128_a2*>(reinterpret_cast<unsigned short*>(p.out) + m * p.ld_out + n + 8 * h) =
                 p.type == 0 ? elem_pack8<0>(a + 8 * h) : elem_pack8<1>(a + 8 * h);
         }
     }
@@ -211,7 +210,7 @@ __global__ __launch_bounds__(64 * KW) void sdmi_mx_direct_kernel(MxGemmDev p) {
                 const int j = min(i0 + 4 * u + q, pairs - 1), step = wave + (j / rows) * KW, r = j % rows;
                 const int64_t k0 = (int64_t)step * MX_KSTEP + row * 8;
                 at[u] = step * rows + r;
-                mx_load8<SRC>(x + r * p.ldx + k0, (int)max((int64_t)0, min((int64_t)8, p.K - k0)), p.vec_x, f[u]);
+                mx_load8<SRC>(x + r * p.ldx + k0, (int)max((int64_t)0, min((int64_t)8, p.K - k0)), f[u]);
             }
 #pragma unroll
             for (int u = 0; u < AT; ++u) {
@@ -511,12 +510,11 @@ extern "C" int sdmi_mx_pack_linear(const void* w, int64_t ldw, int64_t N, int64_
     if (!aligned16(codes) || !aligned16(scales)) return SDMI_ERR_ALIGNMENT;
     const int64_t n = (N + 63) / 64 * 64 * mx_ksteps(K) * 4, blocks = (n + 255) / 256;
     if (blocks >= ((int64_t)1 << 31)) return SDMI_ERR_BAD_ARG;
-    const int vec = aligned16(w) && ldw % (t == 2 ? 4 : 8) == 0;
     hipStream_t st = (hipStream_t)stream;
     unsigned char *c = (unsigned char*)codes, *s = (unsigned char*)scales;
-    if (t == 0) sdmi_mx_pack_kernel<0><<<(unsigned)blocks, 256, 0, st>>>((const unsigned short*)w, ldw, N, K, c, s, vec);
-    else if (t == 1) sdmi_mx_pack_kernel<1><<<(unsigned)blocks, 256, 0, st>>>((const unsigned short*)w, ldw, N, K, c, s, vec);
-    else sdmi_mx_pack_kernel<2><<<(unsigned)blocks, 256, 0, st>>>((const float*)w, ldw, N, K, c, s, vec);
+    if (t == 0) sdmi_mx_pack_kernel<0><<<(unsigned)blocks, 256, 0, st>>>((const unsigned short*)w, ldw, N, K, c, s);
+    else if (t == 1) sdmi_mx_pack_kernel<1><<<(unsigned)blocks, 256, 0, st>>>((const unsigned short*)w, ldw, N, K, c, s);
+    else sdmi_mx_pack_kernel<2><<<(unsigned)blocks, 256, 0, st>>>((const float*)w, ldw, N, K, c, s);
     SDMI_CHECK_LAUNCH();
     return SDMI_OK;
 }
@@ -628,7 +626,6 @@ extern "C" int sdmi_mx_gemm(const sdmi_mx_gemm_args* a, void* stream) {
     if (mx_fused(a)) {
         src = mx_src_type(a->x_dtype);
         d.x = a->x; d.ldx = a->ldx;
-        d.vec_x = aligned16(a->x) && a->ldx % (src == 2 ? 4 : 8) == 0;
     } else if (a->x) {
         unsigned char* const ws = (unsigned char*)a->workspace;
         unsigned char* const xs = ws + up256(a->M * mx_row_bytes(a->K, a->fmt));
@@ -640,7 +637,5 @@ extern "C" int sdmi_mx_gemm(const sdmi_mx_gemm_args* a, void* stream) {
     d.bias = a->bias; d.res = a->res; d.out = a->out;
     d.M = a->M; d.N = a->N; d.K = a->K; d.ksteps = mx_ksteps(a->K); d.ld_res = a->ld_res; d.ld_out = a->ld_out;
     d.type = type;
-    d.vec_out = aligned16(a->out) && a->ld_out % (type == 2 ? 4 : 8) == 0 && aligned16(a->bias) &&
-                (!a->res || (aligned16(a->res) && a->ld_res % (type == 2 ? 4 : 8) == 0));
     return a->fmt == SDMI_MX_FP8 ? mx_launch<SDMI_MX_FP8>(d, mx_kind(a), src, (hipStream_t)stream) : mx_launch<SDMI_MX_FP4>(d, mx_kind(a), src, (hipStream_t)stream);
 }
