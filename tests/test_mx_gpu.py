@@ -165,10 +165,10 @@ def test_gated(dev, act, fmt, rows, c, dtype, pad):
 
 @pytest.mark.parametrize("act", ["gelu", "silu"])
 def test_gate_far_values(dev, act):
-    """Gates far out: the identity on the right, nothing (below the smallest normal fp32) on the left, NaN through."""
-    b = torch.tensor([40.0, 1e4, 1e30, -100.0, -1e4, -1e30, 0.0, float("nan")])
-    y = ops().gated(torch.cat([torch.ones(8), b]).view(1, 16).to(dev), act=act).cpu().view(-1)
-    assert torch.equal(y[:3], b[:3]) and bool((y[3:7].abs() < 2.0 ** -126).all()) and bool(torch.isnan(y[7]))
+    """Gates far out: the identity on the right to infinity, nothing (below the smallest normal fp32) on the left, NaN through."""
+    b = torch.tensor([40.0, 1e4, 1e30, float("inf"), -100.0, -1e4, -1e30, 0.0, float("nan")])
+    y = ops().gated(torch.cat([torch.ones(9), b]).view(1, 18).to(dev), act=act).cpu().view(-1)
+    assert torch.equal(y[:4], b[:4]) and bool((y[4:8].abs() < 2.0 ** -126).all()) and bool(torch.isnan(y[8]))
 
 
 # ----------------------------------------------------------------------------- the product
