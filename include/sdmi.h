@@ -430,7 +430,7 @@ int sdmi_image_to_u8(const float* x, uint8_t* out, int32_t nb, int32_t C, int64_
  * rows == 0 is a valid empty call.  Outputs may not overlap inputs.
  *   sdmi_mx_quantize:   [rows, K] -> codes, scales
  *   sdmi_mx_dequantize: the values that codes and scales stand for (bf16 and fp32 hold them exactly, but for bf16's range)
- *   sdmi_rmsnorm:       s = x + res (res NULL: s = x), y = s / sqrt(mean(s^2) + eps) * gamma; s in fp32, stored in x's type
+ *   sdmi_rmsnorm:       s = x + res (res NULL: s = x), y = s / sqrt(mean(s^2) + eps) * gamma; s in fp32, the mean in fp64; s is stored in x's type
  *       to sum_out [rows, C] (required with res, ignored without).  C <= SDMI_RMSNORM_MAX_C.  fmt SDMI_MX_NONE: out is
  *       [rows, C] of out_dtype; else out holds codes, and scales the scales.
  *   sdmi_gated:         y = a * act(b), x = [a | b] with halves of `inner` columns (the order of the GEGLU projection,

@@ -115,7 +115,7 @@ __global__ __launch_bounds__(256) void sdmi_mx_dequantise_kernel(MxElemArgs p) {
 
 // ---- RMS norm ----------------------------------------------------------------------------------------------------------
 // s = x + res (stored in x's type), y = s / sqrt(mean s^2 + eps) * gamma, of the fp32 sum.  TPR threads hold a row in
-// registers, U chunks of 8 values each, so that a row is read once; the sum of squares is an fp32 tree over those threads.
+// registers, U chunks of 8 values each, so that a row is read once.
 struct MxNormArgs {
     const void* x;
     const void* res;           // NULL: s = x
@@ -125,6 +125,7 @@ struct MxNormArgs {
     unsigned char* codes;
     unsigned char* scales;
     int64_t ldx, ld_res, rows, C;
+    double inv_c;
     float eps;
 };
 
@@ -132,7 +133,7 @@ template <int T, int FMT, int TO, int TPR, int U>
 __global__ __launch_bounds__(256) void sdmi_rmsnorm_kernel(MxNormArgs p) {
     typedef typename MxElem<T>::type E;
     constexpr int RPB = 256 / TPR;
-    __shared__ float part[RPB][TPR / 64];
+    __shared__ double part[RPB][TPR / 64];
     const int t = threadIdx.x % TPR, r = threadIdx.x / TPR, lane = threadIdx.x & 63;
     // Workgroups go round the 8 XCDs; of every 64 each XCD takes 8 neighbours, whose codes and scales share cache lines of its
     // L2 (16384 x 5120 with residual and 8-bit output: 129 -> 120 us; runs of 2 and 32 the same or slower, one run an XCD 152:
@@ -162,21 +163,27 @@ __global__ __launch_bounds__(256) void sdmi_rmsnorm_kernel(MxNormArgs p) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[u][j] += q[u][j];
     }
-    float ss = 0.0f;
+    // In fp64, which costs nothing beside the bytes: every value of a row is scaled by the same number, so an error in it moves
+    // all of them towards the same side of the codes' rounding borders; and no square overflows or vanishes.
+    double ss = 0.0;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss = fmaf(f[u][j], f[u][j], ss);
+        for (int j = 0; j < 8; ++j) ss = fma((double)f[u][j], (double)f[u][j], ss);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
     if constexpr (TPR > 64) {
         if (lane == 0) part[r][t >> 6] = ss;
         __syncthreads();
-        ss = 0.0f;
+        ss = 0.0;
 #pragma unroll
         for (int w = 0; w < TPR / 64; ++w) ss += part[r][w];
     }
-    const float rstd = 1.0f / sqrtf(ss / (float)p.C + p.eps);
+    // 1 / sqrt(v), one Newton step from the approximation, as the sum of two fp32 numbers
+    const double v = ss * p.inv_c + (double)p.eps;
+    double r1 = __builtin_amdgcn_rsq(v);
+    if (v > 0.0 && v < 1e300) r1 *= fma(-0.5 * v * r1, r1, 1.5);
+    const float r0 = (float)r1, lo = r0 < 3e38f ? (float)(r1 - (double)r0) : 0.0f;
     const int64_t nsteps = mx_ksteps(p.C);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -187,7 +194,7 @@ __global__ __launch_bounds__(256) void sdmi_rmsnorm_kernel(MxNormArgs p) {
         float gm[8];
         mx_load8<2>(p.gamma + c0, n, gm);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) gm[j] *= f[u][j] * rstd;
+        for (int j = 0; j < 8; ++j) gm[j] *= fmaf(f[u][j], r0, f[u][j] * lo);
         if constexpr (FMT < 0) {
             if (row < p.rows && n > 0)
                 mx_store8<TO>(reinterpret_cast<typename MxElem<TO>::type*>(p.out) + row * p.C + c0, n, gm);
@@ -334,7 +341,7 @@ extern "C" int sdmi_rmsnorm(const void* x, int64_t ldx, const void* res, int64_t
     MxNormArgs a = {};
     a.x = x; a.res = res; a.gamma = gamma; a.sum_out = res ? sum_out : nullptr; a.out = out;
     a.codes = (unsigned char*)out; a.scales = (unsigned char*)scales;
-    a.ldx = ldx; a.ld_res = ld_res; a.rows = rows; a.C = C; a.eps = eps;
+    a.ldx = ldx; a.ld_res = ld_res; a.rows = rows; a.C = C; a.inv_c = 1.0 / (double)C; a.eps = eps;
     hipStream_t st = (hipStream_t)stream;
     return t == 0 ? norm_type<0>(a, fmt, to, st) : t == 1 ? norm_type<1>(a, fmt, to, st) : norm_type<2>(a, fmt, to, st);
 }

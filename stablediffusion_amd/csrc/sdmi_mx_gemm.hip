@@ -316,13 +316,15 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void sdmi_mx_tiled_kernel(MxGemm
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WGN, wn = wave % WGN, row = lane & 15, q = lane >> 4;
 
-    // Workgroups go round the 8 XCDs; each XCD takes a run of consecutive tiles, and a run walks 8 token tiles before the next
-    // column tile, so that the tiles an XCD works on together share their operands in its L2.
+    // Workgroups go round the 8 XCDs; each XCD takes a run of consecutive tiles, and a run walks BAND token tiles before the next
+    // column tile, so that the tiles an XCD works on together - 32 of 256 x 256, 64 of the smaller ones - are a compact patch
+    // and share their operands in its L2 (8192 x 8192 x 8192 in 8 bits: BAND 2 362 us, 4 354, 8 363, 16 369, 32 405).
     const unsigned tm = (unsigned)((p.M + BM - 1) / BM), tn = (unsigned)((p.N + T::BN - 1) / T::BN), total = tm * tn;
     const unsigned xcd = blockIdx.x & 7, each = total >> 3, more = total & 7;
     const unsigned id = (xcd < more ? xcd * (each + 1) : more + xcd * each) + (blockIdx.x >> 3);
-    const unsigned band = id / (8 * tn), height = min(8u, tm - band * 8), in_band = id - band * 8 * tn;
-    const int64_t m0 = (int64_t)(band * 8 + in_band % height) * BM;
+    constexpr unsigned BAND = BM == 256 ? 4 : 8;
+    const unsigned band = id / (BAND * tn), height = min(BAND, tm - band * BAND), in_band = id - band * BAND * tn;
+    const int64_t m0 = (int64_t)(band * BAND + in_band % height) * BM;
     const int64_t g0 = (int64_t)(in_band / height) * WGN, groups = (p.N + 63) >> 6;
 
     const int nk = (int)p.ksteps;
@@ -535,17 +537,18 @@ static bool mx_args_ok(const sdmi_mx_gemm_args* a) {
 //     48 x  5120 x 5120: direct 16 x 64  7.2, direct 48 x 32  8.7, direct 16 x 32  8.7, tiled 64 x 128 15.2
 //    256 x  1280 x 1280: direct 48 x 32  5.0, tiled 64 x 128  6.6, tiled 128 x 128  8.8
 //    512 x  5120 x 1280: tiled 64 x 128  9.3, tiled 128 x 128  9.5, tiled 256 x 256 18.3, direct 64 x 32 23.4
+//   1024 x  5120 x 5120: tiled 128 x 256 28.9, tiled 128 x 128 32.3, tiled 64 x 128 33.2, tiled 256 x 256 48.8
 //   4096 x  5120 x 5120: tiled 128 x 128 86.9, tiled 256 x 256 102.6 (320 tiles: two rounds), tiled 64 x 128 105.7
-//   8192 x  8192 x 8192: tiled 256 x 256  366, tiled 128 x 128  439
+//   8192 x  8192 x 8192: tiled 256 x 256  354, tiled 128 x 128  439
 // Parts of K in several workgroups of a tiled kernel and a second launch that joins them were measured too (two and four parts)
 // and won by 6 % at most, at one size: the workgroups of a direct kernel split K among their waves already.
-enum MxKind { MX_D16x32, MX_D16x64, MX_D48x32, MX_D64x32, MX_T64x128, MX_T128x128, MX_T256x256, MX_KINDS };
+enum MxKind { MX_D16x32, MX_D16x64, MX_D48x32, MX_D64x32, MX_T64x128, MX_T128x128, MX_T128x256, MX_T256x256, MX_KINDS };
 struct MxCost { int rows, cols, unit; struct { float fixed, first, more; } us[2]; };      // [0]: 8-bit activations, [1]: 4-bit
 static const MxCost MX_COST[MX_KINDS] = {
     {16, 32, 8, {{2.76f, 0.482f, 0.591f}, {2.68f, 0.405f, 0.518f}}},    {16, 64, 8, {{2.69f, 0.717f, 0.983f}, {2.78f, 0.570f, 0.899f}}},
     {48, 32, 8, {{2.96f, 0.835f, 1.476f}, {2.97f, 0.579f, 1.127f}}},    {64, 32, 8, {{2.97f, 1.072f, 1.908f}, {3.11f, 0.691f, 1.431f}}},
     {64, 128, 1, {{3.84f, 0.278f, 0.276f}, {3.80f, 0.270f, 0.204f}}},   {128, 128, 1, {{4.37f, 0.410f, 0.432f}, {4.28f, 0.321f, 0.322f}}},
-    {256, 256, 1, {{7.88f, 1.021f, 1.603f}, {7.99f, 0.638f, 1.196f}}},
+    {128, 256, 1, {{5.00f, 0.590f, 0.730f}, {5.00f, 0.460f, 0.640f}}},  {256, 256, 1, {{7.88f, 1.021f, 1.603f}, {7.99f, 0.638f, 1.196f}}},
 };
 static MxKind mx_kind(const sdmi_mx_gemm_args* a) {
     const int b = a->fmt == SDMI_MX_FP8 ? 0 : 1;
@@ -608,6 +611,7 @@ template <int FMT> static int mx_launch(const MxGemmDev& d, MxKind kind, int src
         case MX_D64x32: return direct_launch<FMT, 4, 2, 8, 1, -1>(d, st);
         case MX_T64x128: return tiled_launch<FMT, 64, 2, 2, 4>(d, st);
         case MX_T128x128: return tiled_launch<FMT, 128, 2, 2, ST>(d, st);
+        case MX_T128x256: return tiled_launch<FMT, 128, 2, 4, 4>(d, st);
         default: return tiled_launch<FMT, 256, 2, 4, ST>(d, st);
     }
 }

@@ -8,8 +8,8 @@ import mx_oracle as O
 pytestmark = pytest.mark.gpu
 
 TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
-# fp32 arithmetic of the row-wise operators: the sum of squares is 64 serial terms and a tree of 8 at most, one division, one
-# square root, two products: (72 / 2 + 5) 2^-24 < 2^-18
+# the norm: the sum is taken in fp64, the value is multiplied twice and s is a sum in fp32: 3 2^-24 and the two-part
+# reciprocal root 2^-40, far below the bound that an fp32 sum would need, (72 / 2 + 5) 2^-24 < 2^-18
 NORM_REL = 2.0 ** -18
 # the gate, |x| <= 12: the exponential's argument x^2 / 2 <= 72 is rounded once, and once more when it is taken to base 2:
 # 144 2^-24 relative in the result; the fitted polynomial adds 11 2^-24, the reciprocal and the products 10: < 2^-16
@@ -144,6 +144,18 @@ def test_rmsnorm_rows_of_zeros_poison_and_types(dev, fmt):
                NORM_REL, torch.float16)
         assert bool(torch.isnan(o.rmsnorm(x[1:2].to(dev), gamma, 0.0)).all())      # 0 / 0, as the formula has it
     assert o.rmsnorm(x[:0].to(dev), gamma).shape == (0, 320)
+
+
+@pytest.mark.parametrize("scale", [1e-36, 1e-25, 1.0, 1e25, 1e36])
+def test_rmsnorm_of_far_magnitudes(dev, scale):
+    """Rows whose squares leave fp32 on either side: the norm of a scaled row is that of the row (eps 0)."""
+    x = (data(5, 700, 3, "f32", loud=False).double() * scale).float()
+    want = O.rmsnorm(x.double(), torch.ones(700).double(), 0.0)
+    within(ops().rmsnorm(x.to(dev), torch.ones(700, device=dev), 0.0), want, NORM_REL, torch.float32)
+    bad = x.clone()
+    bad[2, 5] = float("inf")
+    y = ops().rmsnorm(bad.to(dev), torch.ones(700, device=dev), 0.0).cpu()
+    assert bool(torch.isnan(y[2, 5])) and int(y[2].nan_to_num().count_nonzero()) == 0 and bool(torch.isfinite(y[[0, 1, 3, 4]]).all())
 
 
 # ----------------------------------------------------------------------------- gated activation
