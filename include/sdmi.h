@@ -440,6 +440,7 @@ int sdmi_image_to_u8(const float* x, uint8_t* out, int32_t nb, int32_t C, int64_
 #define SDMI_MX_FP8 1
 #define SDMI_MX_FP4 2
 #define SDMI_RMSNORM_MAX_C 16384
+#define SDMI_MX_ALGOS 8
 int64_t sdmi_mx_codes_bytes(int64_t rows, int64_t K, int32_t fmt);
 int64_t sdmi_mx_scales_bytes(int64_t rows, int64_t K);
 int sdmi_mx_quantize(const void* x, int64_t ldx, int64_t rows, int64_t K, int32_t dtype, void* codes, void* scales,
@@ -475,7 +476,9 @@ typedef struct sdmi_mx_gemm_args {
     int64_t ldx, ld_res, ld_out;
     int32_t x_dtype, out_dtype;
     int32_t fmt;             /* of the activations */
-    int32_t reserved;        /* 0 */
+    int32_t algo;            /* 0: the library picks the kernel; 1 ... SDMI_MX_ALGOS pins one (tests, measurements): the direct
+                                kernels of 16 x 32, 16 x 64, 48 x 32, 64 x 32 outputs a workgroup, the tiled ones of 64 x 128,
+                                128 x 128, 128 x 256, 256 x 256 */
 } sdmi_mx_gemm_args;
 int64_t sdmi_mx_gemm_workspace_bytes(const sdmi_mx_gemm_args* args);   /* -1: sizes that sdmi_mx_gemm refuses */
 int sdmi_mx_gemm(const sdmi_mx_gemm_args* args, void* stream);

@@ -525,7 +525,7 @@ static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
 static bool mx_args_ok(const sdmi_mx_gemm_args* a) {
     if (!a || a->M < 0 || a->N <= 0 || a->K <= 0 || a->M >= ((int64_t)1 << 31) || a->N > MX_MAX_DIM || a->K > MX_MAX_DIM) return false;
-    if (a->fmt != SDMI_MX_FP8 && a->fmt != SDMI_MX_FP4) return false;
+    if ((a->fmt != SDMI_MX_FP8 && a->fmt != SDMI_MX_FP4) || a->algo < 0 || a->algo > SDMI_MX_ALGOS) return false;
     return !a->x || (mx_src_type(a->x_dtype) >= 0 && a->ldx >= a->K);
 }
 
@@ -550,7 +550,9 @@ static const MxCost MX_COST[MX_KINDS] = {
     {64, 128, 1, {{3.84f, 0.278f, 0.276f}, {3.80f, 0.270f, 0.204f}}},   {128, 128, 1, {{4.37f, 0.410f, 0.432f}, {4.28f, 0.321f, 0.322f}}},
     {128, 256, 1, {{5.00f, 0.590f, 0.730f}, {5.00f, 0.460f, 0.640f}}},  {256, 256, 1, {{7.88f, 1.021f, 1.603f}, {7.99f, 0.638f, 1.196f}}},
 };
+static_assert(MX_KINDS == SDMI_MX_ALGOS, "sdmi_mx_gemm_args.algo");
 static MxKind mx_kind(const sdmi_mx_gemm_args* a) {
+    if (a->algo) return (MxKind)(a->algo - 1);
     const int b = a->fmt == SDMI_MX_FP8 ? 0 : 1;
     int best = MX_T256x256;
     double least = 0;
@@ -568,7 +570,7 @@ static MxKind mx_kind(const sdmi_mx_gemm_args* a) {
 // 1 x 10240 x 5120: 8.8 us against 2.5 for the quantisation and 8.5 (4 rows x 5120 x 2560: 4.7 against 9.1); every workgroup
 // quantises all of the rows, so that it does not pay for many of them.
 static bool mx_fused(const sdmi_mx_gemm_args* a) {
-    return a->x && a->M <= MX_FUSED_ROWS && a->M * mx_ksteps(a->K) * (mx_row_bytes(128, a->fmt) + 4) <= 48 * 1024;
+    return a->x && !a->algo && a->M <= MX_FUSED_ROWS && a->M * mx_ksteps(a->K) * (mx_row_bytes(128, a->fmt) + 4) <= 48 * 1024;
 }
 
 extern "C" int64_t sdmi_mx_gemm_workspace_bytes(const sdmi_mx_gemm_args* a) {

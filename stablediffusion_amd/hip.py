@@ -15,6 +15,7 @@ SDMI_OK = 0
 DTYPE_BF16, DTYPE_F16, DTYPE_F32_PLANES, DTYPE_F16_TO_BF16, DTYPE_F32 = 0, 1, 2, 3, 4
 MX_NONE, MX_FP8, MX_FP4 = 0, 1, 2
 RMSNORM_MAX_C = 16384
+MX_ALGOS = 8
 
 
 class SdmiError(RuntimeError):
@@ -80,7 +81,7 @@ class MxGemmArgs(C.Structure):
         ("x", C.c_void_p), ("x_codes", C.c_void_p), ("x_scales", C.c_void_p), ("w_codes", C.c_void_p), ("w_scales", C.c_void_p),
         ("bias", C.c_void_p), ("res", C.c_void_p), ("out", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
         ("M", C.c_int64), ("N", C.c_int64), ("K", C.c_int64), ("ldx", C.c_int64), ("ld_res", C.c_int64), ("ld_out", C.c_int64),
-        ("x_dtype", C.c_int32), ("out_dtype", C.c_int32), ("fmt", C.c_int32), ("reserved", C.c_int32),
+        ("x_dtype", C.c_int32), ("out_dtype", C.c_int32), ("fmt", C.c_int32), ("algo", C.c_int32),
     ]
 
 

@@ -854,6 +854,10 @@ class MxTensor:
     def device(self):
         return self.buf.device
 
+    def record_stream(self, stream):
+        """As torch.Tensor.record_stream: for a tensor that another stream than its own reads."""
+        self.buf.record_stream(stream)
+
 
 class PackedMxWeight:
     """[N, K] linear weights in 4 bits with one scale per 32 (sdmi_mx_pack_linear), and the fp32 bias or None."""
@@ -1035,22 +1039,13 @@ def pack_linear_mx(weight, bias=None):
     return pw
 
 
-def _mx_scratch(nbytes, device):
-    """_scratch() for `device`, which need not be the current one."""
-    index = device.index
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            return _scratch(nbytes, device)
-    buf = _SCRATCH.get((index, torch._C._cuda_getCurrentRawStream(index)))
-    if buf is not None and buf.numel() >= nbytes and not torch.cuda.is_current_stream_capturing():
-        return buf
-    return _scratch(nbytes, device)
+FORCE_MX_ALGO = 0     # development aid / tests: sdmi_mx_gemm_args.algo
 
 
 @functools.lru_cache(maxsize=4096)
-def _mx_gemm_workspace(m, n, k, ldx, x_dt, fmt):
+def _mx_gemm_workspace(m, n, k, ldx, x_dt, fmt, algo):
     a = hip.MxGemmArgs()
-    a.M, a.N, a.K, a.ldx, a.x_dtype, a.fmt = m, n, k, ldx, x_dt, fmt
+    a.M, a.N, a.K, a.ldx, a.x_dtype, a.fmt, a.algo = m, n, k, ldx, x_dt, fmt, algo
     a.x = 16 if x_dt >= 0 else None          # (only whether there is one counts)
     return hip.lib().sdmi_mx_gemm_workspace_bytes(C.byref(a))
 
@@ -1086,9 +1081,11 @@ def linear_mx(x, pw, fmt=None, res=None, out_dtype=None):
         return out
     a.M, a.N, a.K, a.fmt, a.ld_out = m, n, k, code, n
     a.w_codes, a.w_scales, a.out, a.bias = pw.codes_ptr, pw.scales_ptr, out.data_ptr(), pw.bias_ptr
-    nbytes = _mx_gemm_workspace(m, n, k, ldx, x_dt, code)
+    a.algo = FORCE_MX_ALGO
+    nbytes = _mx_gemm_workspace(m, n, k, ldx, x_dt, code, FORCE_MX_ALGO)
     if nbytes > 0:
-        ws = _mx_scratch(nbytes, dev)
+        # of this call alone: the call makes two launches, and another thread's on the same stream may come between them
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
     _mx_call(hip.lib().sdmi_mx_gemm, "sdmi_mx_gemm", dev, C.byref(a))
     return out

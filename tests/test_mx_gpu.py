@@ -241,6 +241,51 @@ def test_linear_mx(dev, fmt, m, n, k):
     assert bool(((y32.double().cpu() - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("algo", range(1, 9))
+def test_every_kernel(dev, monkeypatch, fmt, algo):
+    """Each kernel pinned, at 1 ... 9 k-steps (fewer than its ring holds, and more), tokens and columns that fill no tile and
+    one column past one, with a bias and a residual; and the same call again, bit for bit."""
+    o = ops()
+    monkeypatch.setattr(o, "FORCE_MX_ALGO", algo)
+    for i, (m, n, k) in enumerate([(1, 1, 1), (2, 70, 128), (300, 257, 200), (257, 300, 384), (64, 520, 512), (33, 128, 640), (129, 65, 700),
+                                   (513, 260, 896), (70, 600, 1024), (260, 130, 1100)]):
+        x, w = data(m, k, i, "f32", loud=i % 2 == 0), torch.randn(n, k, generator=torch.Generator().manual_seed(i)) * k ** -0.5
+        g = torch.Generator().manual_seed(50 + i)
+        bias, res = (torch.randn(n, generator=g), torch.randn(m, n, generator=g)) if i % 3 else (None, None)
+        pw, q = o.pack_linear_mx(w.to(dev), None if bias is None else bias.to(dev)), o.mx_quantize(x.to(dev), fmt)
+        y = o.linear_mx(q, pw, res=None if res is None else res.to(dev), out_dtype=torch.float32)
+        want, tol = product(O.values(x.double(), fmt), O.values(w.double(), "mxfp4"), fmt, bias, res)
+        off = (y.double().cpu() - want).abs()
+        assert bool((off <= tol).all()), f"{(m, n, k)}: largest excess {float((off - tol).max()):.3e}"
+        for _ in range(3):
+            assert torch.equal(o.linear_mx(q, pw, res=None if res is None else res.to(dev), out_dtype=torch.float32), y), (m, n, k)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+def test_kernels_agree_on_large_products(dev, monkeypatch, fmt):
+    """Many tiles and k-steps at once, where a fill that is not waited for would show: the tiled kernels against each other (the
+    same order of sums) and against the direct one (another order), several times."""
+    o = ops()
+    m, n, k = 2100, 2600, 2700
+    q = o.mx_quantize(data(m, k, 1, "bf16", loud=False).to(dev), fmt)
+    pw = o.pack_linear_mx(torch.randn(n, k, generator=torch.Generator().manual_seed(1)).to(dev) * k ** -0.5)
+
+    def run(algo):
+        monkeypatch.setattr(o, "FORCE_MX_ALGO", algo)
+        return o.linear_mx(q, pw, out_dtype=torch.float32)
+
+    first = run(8)
+    direct = run(4)
+    for algo in (5, 6, 7, 8):
+        for _ in range(5):
+            assert torch.equal(run(algo), first), algo
+    a, b = O.values(data(m, k, 1, "bf16", loud=False).double(), fmt), o.mx_dequantize(q).double().cpu()
+    assert torch.equal(a, b)
+    s = a[:64].abs() @ O.values(torch.randn(n, k, generator=torch.Generator().manual_seed(1)).mul(k ** -0.5).double(), "mxfp4").abs().t()
+    assert bool(((direct - first).double().abs().cpu()[:64] <= 2 * s * ((k + 2) * 2.0 ** -23 + 7 * 2.0 ** -13)).all())
+
+
 @pytest.mark.parametrize("m", [1, 20, 150])
 @pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
 def test_linear_mx_picks_single_elements(dev, fmt, m):
@@ -346,6 +391,29 @@ def test_feed_forward_links(dev, tokens, fmt, act):
         assert bool(((got.double().cpu() - want).abs() <= tol).all())
     hc = h.double().cpu()
     assert O.held_within(av.double(), hc[:, :inner] * O.gate(hc[:, inner:], act), GATE_REL, fmt)
+
+
+def test_calls_of_two_threads_on_one_stream(dev):
+    """A product of plain activations is a quantisation and a product; two threads' calls on one stream keep theirs apart."""
+    import threading
+    o = ops()
+    pw = o.pack_linear_mx(torch.randn(96, 512, generator=torch.Generator().manual_seed(1)).to(dev))
+    xs = [data(200, 512, i).to(dev) for i in range(2)]
+    want = [o.linear_mx(x, pw) for x in xs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        got = [o.linear_mx(xs[i], pw) for _ in range(200)]
+        torch.cuda.synchronize()
+        wrong.extend(1 for y in got if not torch.equal(y, want[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 @pytest.mark.parametrize("m", [1, 40, 300])

@@ -96,7 +96,7 @@ def test_product_refusals(lib):
     assert g() == OK
     assert g(x=None, x_codes=P, x_scales=P) == OK
     for bad in (dict(w_codes=None), dict(w_scales=None), dict(out=None), dict(x=None), dict(x=None, x_codes=P), dict(ldx=63), dict(x_dtype=3),
-                dict(N=0), dict(K=0), dict(M=-1), dict(fmt=0), dict(out_dtype=2), dict(ld_out=63), dict(res=P, ld_res=63), dict(K=(1 << 24) + 1, ldx=1 << 25)):
+                dict(N=0), dict(K=0), dict(M=-1), dict(fmt=0), dict(algo=-1), dict(algo=9), dict(out_dtype=2), dict(ld_out=63), dict(res=P, ld_res=63), dict(K=(1 << 24) + 1, ldx=1 << 25)):
         assert g(**{"M": 4, **bad}) == BAD, bad
     assert lib.sdmi_mx_gemm(None, None) == BAD
     for bad in (dict(w_codes=P + 8), dict(w_scales=P + 2), dict(x=None, x_codes=P + 8, x_scales=P)):
