@@ -145,9 +145,9 @@ __device__ __forceinline__ void mx_store_run(const MxGemmDev& p, int64_t m, int6
 // Few tokens: the weights' bytes are the work, and a workgroup has to have many of them in flight.  It takes NF of a group's
 // four fragments (4 NF columns of every 16) for MT x 16 tokens; its KW waves take every KW-th k-step from memory straight into
 // registers, U k-steps ahead of the ones they multiply, and join their sums through LDS in a fixed order.
-// SRC >= 0: x is a plain matrix of that type (mx_src_type) and at most MX_FUSED_ROWS rows, which every workgroup quantises for
-// itself into LDS while its first weights are on their way: one launch instead of two.
-constexpr int MX_FUSED_ROWS = 4;
+// SRC >= 0: x is a plain matrix of that type (mx_src_type) and few rows (mx_fused), which every workgroup quantises for itself
+// into LDS while its first weights are on their way: one launch instead of two.
+constexpr int MX_FUSED_PAIRS = 16;        // (k-step, row) pairs that a wave quantises: what its lanes load in one go
 
 template <int FMT, int MT, int NF, int KW, int U, int SRC>
 __global__ __launch_bounds__(64 * KW) void sdmi_mx_direct_kernel(MxGemmDev p) {
@@ -193,21 +193,22 @@ __global__ __launch_bounds__(64 * KW) void sdmi_mx_direct_kernel(MxGemmDev p) {
         }
     };
     if (mine > 0) load(0, 0);
+    if (mine > U) load(1, U);
     unsigned char* const own = smem;                       // SRC >= 0: [nk][M][RB] codes, then [nk][M][4] scales
     const int rows = (int)p.M;
     unsigned char* const own_s = smem + nk * rows * RB;
     if constexpr (SRC >= 0) {
         // the wave quantises the k-steps that it alone will read: four (k-step, row) pairs at a time, 16 lanes each, and AT
         // times four on their way together (pairs past the end: the last one again)
-        constexpr int AT = 4;
+        constexpr int AT = MX_FUSED_PAIRS / 4;
         const typename MxElem<SRC>::type* const x = reinterpret_cast<const typename MxElem<SRC>::type*>(p.x);
         const int pairs = mine * rows;
-        for (int i0 = 0; i0 < pairs; i0 += 4 * AT) {
+        if (pairs > 0) {
             float f[AT][8];
             int at[AT];
 #pragma unroll
             for (int u = 0; u < AT; ++u) {
-                const int j = min(i0 + 4 * u + q, pairs - 1), step = wave + (j / rows) * KW, r = j % rows;
+                const int j = min(4 * u + q, pairs - 1), step = wave + (j / rows) * KW, r = j % rows;
                 const int64_t k0 = (int64_t)step * MX_KSTEP + row * 8;
                 at[u] = step * rows + r;
                 mx_load8<SRC>(x + r * p.ldx + k0, (int)max((int64_t)0, min((int64_t)8, p.K - k0)), f[u]);
@@ -249,10 +250,10 @@ __global__ __launch_bounds__(64 * KW) void sdmi_mx_direct_kernel(MxGemmDev p) {
         }
     };
     for (int i = 0; i < mine; i += 2 * U) {
-        if (i + U < mine) load(1, i + U);
         multiply(0, i);
         if (i + 2 * U < mine) load(0, i + 2 * U);
         if (i + U < mine) multiply(1, i + U);
+        if (i + 3 * U < mine) load(1, i + 3 * U);
     }
     if constexpr (SRC >= 0) __syncthreads();               // the codes' place becomes that of the sums
     f32x4* const part = reinterpret_cast<f32x4*>(smem);
@@ -566,11 +567,11 @@ static MxKind mx_kind(const sdmi_mx_gemm_args* a) {
     return (MxKind)best;
 }
 
-// The direct kernel quantises plain activations itself: one launch for up to MX_FUSED_ROWS rows whose codes fit its LDS.
-// 1 x 10240 x 5120: 8.8 us against 2.5 for the quantisation and 8.5 (4 rows x 5120 x 2560: 4.7 against 9.1); every workgroup
-// quantises all of the rows, so that it does not pay for many of them.
+// The direct kernel quantises plain activations itself where a wave's share is one round of loads.  On the GPU alone the two
+// ways are near each other - 8 x 1280 x 1280 5.0 us fused, 5.8 as quantisation and product; 1 x 5120 x 5120 7.5 and 8.4; 1 x
+// 10240 x 5120 9.2 and 10.3; a second round of loads costs 2 us - and a launch less is 3 us less of the caller's time.
 static bool mx_fused(const sdmi_mx_gemm_args* a) {
-    return a->x && !a->algo && a->M <= MX_FUSED_ROWS && a->M * mx_ksteps(a->K) * (mx_row_bytes(128, a->fmt) + 4) <= 48 * 1024;
+    return a->x && !a->algo && a->M <= MX_FUSED_PAIRS && a->M * ((mx_ksteps(a->K) + 7) / 8) <= MX_FUSED_PAIRS;
 }
 
 extern "C" int64_t sdmi_mx_gemm_workspace_bytes(const sdmi_mx_gemm_args* a) {
@@ -605,6 +606,8 @@ template <int FMT, int MT, int NF, int KW, int U, int SRC> static int direct_lau
 
 template <int FMT> static int mx_launch(const MxGemmDev& d, MxKind kind, int src, hipStream_t st) {
     constexpr int ST = FMT == SDMI_MX_FP8 ? 3 : 4;
+    // quantising: 64 columns a workgroup where 32 would make more than one for each CU (1 x 10240 x 2560: 8.4 -> 7.1 us)
+    if (src >= 0 && d.N > 256 * 32) return src == 0 ? direct_launch<FMT, 1, 4, 8, 2, 0>(d, st) : src == 1 ? direct_launch<FMT, 1, 4, 8, 2, 1>(d, st) : direct_launch<FMT, 1, 4, 8, 2, 2>(d, st);
     if (src >= 0) return src == 0 ? direct_launch<FMT, 1, 2, 8, 2, 0>(d, st) : src == 1 ? direct_launch<FMT, 1, 2, 8, 2, 1>(d, st) : direct_launch<FMT, 1, 2, 8, 2, 2>(d, st);
     switch (kind) {
         case MX_D16x32: return direct_launch<FMT, 1, 2, 8, 2, -1>(d, st);

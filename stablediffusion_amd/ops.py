@@ -915,17 +915,11 @@ def _mx_rows(t, name):
     return rows, k, ld
 
 
-def _mx_same(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise hip.SdmiError(f"{name} is on {t.device}, the input on {device}")
-
-
 def _mx_call(fn, what, device, *args):
     """fn(*args, stream) on `device` and its current stream.  Operators of a few microseconds: the raw handle is asked for
     where torch.cuda.current_stream() would make an object first (0.1 us for 2.8)."""
     index = device.index
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         st = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
@@ -974,8 +968,9 @@ def rmsnorm(x, gamma, eps=1e-6, res=None, fmt=None, out_dtype=None):
         if res.dtype != x.dtype or res.shape != x.shape:
             raise hip.SdmiError(f"rmsnorm: res is {res.dtype} {tuple(res.shape)}, x {x.dtype} {tuple(x.shape)}")
         ld_res = _mx_rows(res, "res")[2]
-        s = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    _mx_same(x.device, gamma=gamma, res=res)
+        s = torch.empty_like(x, memory_format=torch.contiguous_format)
+    if gamma.device != x.device or (res is not None and res.device != x.device):
+        raise hip.SdmiError(f"rmsnorm: gamma and res have to be on x's device, {x.device}")
     if fmt is None:
         y = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
         out, scales, code, odt = y.data_ptr(), None, hip.MX_NONE, _mx_dt(y.dtype, "rmsnorm out_dtype")
@@ -1031,7 +1026,8 @@ def pack_linear_mx(weight, bias=None):
         b = _src(bias).clone()          # the packed layer owns its parameters: the caller's tensor may change
         if b.shape != (n,):
             raise hip.SdmiError(f"pack_linear_mx: bias {tuple(bias.shape)} for {n} outputs")
-    _mx_same(w.device, bias=b)
+    if b is not None and b.device != w.device:
+        raise hip.SdmiError(f"pack_linear_mx: bias is on {b.device}, the weight on {w.device}")
     lib = hip.lib()
     pw = PackedMxWeight(torch.empty(lib.sdmi_mx_weight_codes_bytes(n, k), dtype=torch.uint8, device=w.device),
                         torch.empty(lib.sdmi_mx_weight_scales_bytes(n, k), dtype=torch.uint8, device=w.device), b, n, k)
@@ -1070,7 +1066,8 @@ def linear_mx(x, pw, fmt=None, res=None, out_dtype=None):
         raise hip.SdmiError(f"linear_mx: K mismatch ({k} vs packed {pw.k})")
     n = pw.n_out
     shape = (*x.shape[:-1], n)
-    _mx_same(dev, weight=pw.codes, res=res)
+    if pw.codes.device != dev or (res is not None and res.device != dev):
+        raise hip.SdmiError(f"linear_mx: the weight and res have to be on x's device, {dev}")
     a.out_dtype = _mx_dt(out_dtype, "linear_mx out_dtype")
     if res is not None:
         if res.dtype != out_dtype or res.shape != shape:
