@@ -531,25 +531,30 @@ static bool mx_args_ok(const sdmi_mx_gemm_args* a) {
 }
 
 // Which kernel runs a product: the cheapest by a model of rounds.  A kernel's workgroups take `rows` x `cols` of the output; a
-// launch costs `fixed` us, a unit of K `first` for the first workgroup on each of the 256 CUs and `more` for every further
-// round of them.  (Direct kernels: the unit is eight k-steps, one for each wave; tiled ones: one k-step.)  Least squares over a
-// sweep of 1 ... 4096 rows and (N, K) of 640 x 640, 1280 x 1280, 5120 x 1280, 1280 x 5120, 5120 x 5120 and 10240 x 2560, every
-// kernel at every size; the kernel it picks is the fastest measured one, or within 14 % of it.  Examples in us, 8-bit activations:
-//     48 x  5120 x 5120: direct 16 x 64  7.2, direct 48 x 32  8.7, direct 16 x 32  8.7, tiled 64 x 128 15.2
-//    256 x  1280 x 1280: direct 48 x 32  5.0, tiled 64 x 128  6.6, tiled 128 x 128  8.8
-//    512 x  5120 x 1280: tiled 64 x 128  9.3, tiled 128 x 128  9.5, tiled 256 x 256 18.3, direct 64 x 32 23.4
-//   1024 x  5120 x 5120: tiled 128 x 256 28.9, tiled 128 x 128 32.3, tiled 64 x 128 33.2, tiled 256 x 256 48.8
-//   4096 x  5120 x 5120: tiled 128 x 128 86.9, tiled 256 x 256 102.6 (320 tiles: two rounds), tiled 64 x 128 105.7
-//   8192 x  8192 x 8192: tiled 256 x 256  354, tiled 128 x 128  439
+// launch costs `fixed` us, a unit of K `first` for the first workgroup on each of the 256 CUs, and every further round of them
+// `round` and `more` a unit.  (Direct kernels: the unit is eight k-steps, one for each wave; tiled ones: one k-step.)  Least
+// squares over a sweep of 1 ... 8192 rows and twelve (N, K) from 320 x 320 to 10240 x 5120 and 2560 x 10240, every kernel at
+// every size; the kernel it picks is within 0.8 % of the fastest one on average and 16 % at worst.  Examples, us, 8-bit
+// activations (direct kernels by their outputs a workgroup, D, tiled ones T):
+//     48 x  5120 x 5120: D 16 x 64  7.2, D 48 x 32  8.7, D 16 x 32  8.7, T 64 x 128 15.2
+//    256 x  1280 x 1280: D 48 x 32  5.0, T 64 x 128  6.6, T 128 x 128  8.8
+//    512 x  5120 x 1280: T 64 x 128  9.3, T 128 x 128  9.5, T 256 x 256 18.3, D 64 x 32 23.4
+//   1024 x  5120 x 5120: T 128 x 256 28.9, T 128 x 128 32.3, T 64 x 128 33.2, T 256 x 256 48.8
+//   4096 x  5120 x 5120: T 128 x 128 86.9, T 256 x 256 102.6 (320 tiles: two rounds), T 64 x 128 105.7
+//   8192 x  8192 x 8192: T 256 x 256  354, T 128 x 128  439
 // Parts of K in several workgroups of a tiled kernel and a second launch that joins them were measured too (two and four parts)
 // and won by 6 % at most, at one size: the workgroups of a direct kernel split K among their waves already.
 enum MxKind { MX_D16x32, MX_D16x64, MX_D48x32, MX_D64x32, MX_T64x128, MX_T128x128, MX_T128x256, MX_T256x256, MX_KINDS };
-struct MxCost { int rows, cols, unit; struct { float fixed, first, more; } us[2]; };      // [0]: 8-bit activations, [1]: 4-bit
+struct MxCost { int rows, cols, unit; struct { double fixed, first, round, more; } us[2]; };      // [0]: 8-bit activations, [1]: 4-bit
 static const MxCost MX_COST[MX_KINDS] = {
-    {16, 32, 8, {{2.76f, 0.482f, 0.591f}, {2.68f, 0.405f, 0.518f}}},    {16, 64, 8, {{2.69f, 0.717f, 0.983f}, {2.78f, 0.570f, 0.899f}}},
-    {48, 32, 8, {{2.96f, 0.835f, 1.476f}, {2.97f, 0.579f, 1.127f}}},    {64, 32, 8, {{2.97f, 1.072f, 1.908f}, {3.11f, 0.691f, 1.431f}}},
-    {64, 128, 1, {{3.84f, 0.278f, 0.276f}, {3.80f, 0.270f, 0.204f}}},   {128, 128, 1, {{4.37f, 0.410f, 0.432f}, {4.28f, 0.321f, 0.322f}}},
-    {128, 256, 1, {{5.00f, 0.590f, 0.730f}, {5.00f, 0.460f, 0.640f}}},  {256, 256, 1, {{7.88f, 1.021f, 1.603f}, {7.99f, 0.638f, 1.196f}}},
+    {16, 32, 8, {{3.543, 0.482, 0.376, 0.486}, {3.610, 0.376, 0.301, 0.393}}},
+    {16, 64, 8, {{3.501, 0.715, 0.704, 0.749}, {3.634, 0.576, 0.656, 0.643}}},
+    {48, 32, 8, {{3.619, 0.874, 1.461, 1.094}, {3.741, 0.566, 1.430, 0.727}}},
+    {64, 32, 8, {{3.673, 1.103, 1.782, 1.359}, {3.799, 0.694, 1.764, 0.896}}},
+    {64, 128, 1, {{4.321, 0.268, 1.492, 0.206}, {4.265, 0.266, 1.265, 0.146}}},
+    {128, 128, 1, {{4.763, 0.423, 2.150, 0.354}, {4.751, 0.323, 2.377, 0.233}}},
+    {128, 256, 1, {{5.956, 0.569, 5.441, 0.721}, {6.060, 0.457, 5.347, 0.533}}},
+    {256, 256, 1, {{7.522, 1.071, 8.450, 1.263}, {8.021, 0.658, 9.104, 0.821}}},
 };
 static_assert(MX_KINDS == SDMI_MX_ALGOS, "sdmi_mx_gemm_args.algo");
 static MxKind mx_kind(const sdmi_mx_gemm_args* a) {
@@ -560,7 +565,8 @@ static MxKind mx_kind(const sdmi_mx_gemm_args* a) {
     for (int i = MX_KINDS - 1; i >= 0; --i) {
         const MxCost& c = MX_COST[i];
         const int64_t blocks = (a->M + c.rows - 1) / c.rows * ((a->N + c.cols - 1) / c.cols), rounds = (blocks + 255) / 256;
-        const double cost = c.us[b].fixed + (double)((mx_ksteps(a->K) + c.unit - 1) / c.unit) * (c.us[b].first + (rounds - 1) * (double)c.us[b].more);
+        const double units = (double)((mx_ksteps(a->K) + c.unit - 1) / c.unit);
+        const double cost = c.us[b].fixed + c.us[b].first * units + (double)(rounds - 1) * (c.us[b].round + c.us[b].more * units);
         if (c.unit > 1 && a->M > 65535 * (int64_t)c.rows) continue;      // the direct kernels' grid
         if (i == MX_KINDS - 1 || cost < least) { best = i; least = cost; }
     }
