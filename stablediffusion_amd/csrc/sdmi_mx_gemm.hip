@@ -7,8 +7,10 @@
 //
 // Packed weights: per group of 64 output columns and k-step of 128, four fragments of 64 lanes x 16 bytes, then (in a second
 // buffer) 64 lanes x 4 scale bytes, one for each fragment (the instruction selects the byte).  Fragment f, row 4 g + r holds
-// column 16 g + 4 f + r of its group: the four accumulator quads of a lane are then 16 CONSECUTIVE columns, stored as two
-// 16-byte vectors, and the four lanes of a token write a whole 128-byte line.
+// column 32 (f / 2) + 8 g + 4 (f % 2) + r of its group: the accumulator quads of fragments 0 and 1 (2 and 3) are then 8
+// CONSECUTIVE columns of a lane, 16 bytes of a 16-bit output, and the four lanes of a token store 64 bytes in one piece
+// (fp32 output of 4096 x 10240 x 1280: 86 us, and
+// 98 with 16 consecutive columns a lane, whose 16-byte pieces lie 64 apart).
 #include "sdmi_mx.h"
 #include <type_traits>
 
@@ -39,7 +41,7 @@ __global__ __launch_bounds__(256) void sdmi_mx_pack_kernel(const typename MxElem
     c.z = mx_codes8<SDMI_MX_FP4>(f[2], inv).x;
     c.w = mx_codes8<SDMI_MX_FP4>(f[3], inv).x;
     if (byte == 255u) c = (uint4){0u, 0u, 0u, 0u};
-    const int nl = (int)(n & 63), frag = (nl & 15) >> 2, lane = (int)(kb & 3) * 16 + (nl >> 4) * 4 + (nl & 3);
+    const int nl = (int)(n & 63), frag = (nl >> 5) * 2 + (nl >> 2 & 1), lane = (int)(kb & 3) * 16 + (nl >> 3 & 3) * 4 + (nl & 3);      // (the map above, inverted)
     const int64_t at = (n >> 6) * ksteps + (kb >> 2);
     *reinterpret_cast<uint4*>(codes + at * 4096 + frag * 1024 + lane * 16) = c;
     scales[at * 256 + lane * 4 + frag] = (unsigned char)byte;
@@ -97,53 +99,58 @@ __device__ __forceinline__ void mx_store_quad(const MxGemmDev& p, int64_t m, int
     }
 }
 
-// out[m, n .. n + 16): the four quads of a lane are consecutive columns
-__device__ __forceinline__ void mx_store_run(const MxGemmDev& p, int64_t m, int64_t n, const f32x4* v) {
-    if (m >= p.M) return;
-    if (n + 16 > p.N) {
-#pragma unroll
-        for (int f = 0; f < 4; ++f) mx_store_quad(p, m, n + 4 * f, v[f]);
-        return;
-    }
-    float a[16];
-#pragma unroll
-    for (int f = 0; f < 4; ++f)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) a[4 * f + r] = v[f][r];
-    if (p.bias) {
-#pragma unroll
-        for (int f = 0; f < 4; ++f) {
-            const f32x4 b = *reinterpret_cast<const mx_f128_a4*>(p.bias + n + 4 * f);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) a[4 * f + r] += b[r];
-        }
-    }
+// A lane's four quads of the 64 columns from n on (see the weights' order), for token m.  16-bit residuals come in `res`: those of
+// several tokens are asked for (mx_load_res) before the first is stored - the compiler cannot know that a store to `out` leaves
+// the residuals alone, and would wait for each in turn (4096 x 10240 x 1280:
+// 80 us, and 87 one by one).
+struct MxRes { uint4 v[2]; };
+__device__ __forceinline__ void mx_load_res(const MxGemmDev& p, int64_t m, int64_t n, int q, MxRes& res) {
+    if (!p.res || p.type == 2 || m >= p.M) return;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        float b[8];
+        const int64_t c = n + 32 * h + 8 * q;
+        if (c + 8 <= p.N) res.v[h] = *reinterpret_cast<const mx_u128_a2*>(reinterpret_cast<const unsigned short*>(p.res) + m * p.ld_res + c);
+    }
+}
+__device__ __forceinline__ void mx_store_run(const MxGemmDev& p, int64_t m, int64_t n, int q, const f32x4* v, const MxRes& res) {
+    if (m >= p.M) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int64_t c = n + 32 * h + 8 * q;
+        if (c + 8 > p.N) {
+            mx_store_quad(p, m, c, v[2 * h]);
+            mx_store_quad(p, m, c + 4, v[2 * h + 1]);
+            continue;
+        }
+        float a[8], b[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a[j] = v[2 * h + j / 4][j % 4];
+        if (p.bias) {
+            mx_load8<2>(p.bias + c, 8, b);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) a[j] += b[j];
+        }
         if (p.type == 2) {
             if (p.res) {
-                mx_load8<2>(reinterpret_cast<const float*>(p.res) + m * p.ld_res + n + 8 * h, 8, b);
+                mx_load8<2>(reinterpret_cast<const float*>(p.res) + m * p.ld_res + c, 8, b);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) a[8 * h + j] += b[j];
+                for (int j = 0; j < 8; ++j) a[j] += b[j];
             }
-            mx_store8<2>(reinterpret_cast<float*>(p.out) + m * p.ld_out + n + 8 * h, 8, a + 8 * h);
+            mx_store8<2>(reinterpret_cast<float*>(p.out) + m * p.ld_out + c, 8, a);
         } else {
             if (p.res) {
-                const uint4 r = *reinterpret_cast<const mx_u128_a2*>(reinterpret_cast<const unsigned short*>(p.res) + m * p.ld_res + n + 8 * h);
-                if (p.type == 0) elem_unpack8<0>(r, b); else elem_unpack8<1>(r, b);
+                if (p.type == 0) elem_unpack8<0>(res.v[h], b); else elem_unpack8<1>(res.v[h], b);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) a[8 * h + j] += b[j];
+                for (int j = 0; j < 8; ++j) a[j] += b[j];
             }
-            *reinterpret_cast<mx_u128_a2*>(reinterpret_cast<unsigned short*>(p.out) + m * p.ld_out + n + 8 * h) =
-                p.type == 0 ? elem_pack8<0>(a + 8 * h) : elem_pack8<1>(a + 8 * h);
+            *reinterpret_cast<mx_u128_a2*>(reinterpret_cast<unsigned short*>(p.out) + m * p.ld_out + c) = p.type == 0 ? elem_pack8<0>(a) : elem_pack8<1>(a);
         }
     }
 }
 
 // ---- direct form --------------------------------------------------------------------------------------------------------
 // Few tokens: the weights' bytes are the work, and a workgroup has to have many of them in flight.  It takes NF of a group's
-// four fragments (4 NF columns of every 16) for MT x 16 tokens; its KW waves take every KW-th k-step from memory straight into
+// four fragments for MT x 16 tokens; its KW waves take every KW-th k-step from memory straight into
 // registers, U k-steps ahead of the ones they multiply, and join their sums through LDS in a fixed order.
 // SRC >= 0: x is a plain matrix of that type (mx_src_type) and few rows (mx_fused), which every workgroup quantises for itself
 // into LDS while its first weights are on their way: one launch instead of two.
@@ -266,7 +273,8 @@ __global__ __launch_bounds__(64 * KW) void sdmi_mx_direct_kernel(MxGemmDev p) {
         f32x4 v = part[t * 64 + lane];
 #pragma unroll
         for (int k = 1; k < KW; ++k) v += part[(k * MT * NF + t) * 64 + lane];
-        mx_store_quad(p, m0 + t / NF * 16 + row, grp * 64 + 16 * q + 4 * (f0 + t % NF), v);
+        const int f = f0 + t % NF;
+        mx_store_quad(p, m0 + t / NF * 16 + row, grp * 64 + 32 * (f >> 1) + 8 * q + 4 * (f & 1), v);
     }
 }
 
@@ -494,10 +502,16 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void sdmi_mx_tiled_kernel(MxGemm
     }
     step(std::false_type(), even, odd, s);
 
-    const int64_t n = (g0 + wn) * 64 + 16 * q;
-    if (n >= p.N) return;
+    constexpr int TOGETHER = T::MF == 8 ? 1 : T::MF;                             // (128 accumulators leave no room for more)
 #pragma unroll
-    for (int mi = 0; mi < T::MF; ++mi) mx_store_run(p, m0 + arow + mi * 16, n, acc[mi]);
+    for (int m1 = 0; m1 < T::MF; m1 += TOGETHER) {
+        MxRes res[TOGETHER];
+#pragma unroll
+        for (int i = 0; i < TOGETHER; ++i) mx_load_res(p, m0 + arow + (m1 + i) * 16, (g0 + wn) * 64, q, res[i]);
+#pragma unroll
+        for (int i = 0; i < TOGETHER; ++i) mx_store_run(p, m0 + arow + (m1 + i) * 16, (g0 + wn) * 64, q, acc[m1 + i], res[i]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------
