@@ -547,28 +547,29 @@ static bool mx_args_ok(const sdmi_mx_gemm_args* a) {
 // Which kernel runs a product: the cheapest by a model of rounds.  A kernel's workgroups take `rows` x `cols` of the output; a
 // launch costs `fixed` us, a unit of K `first` for the first workgroup on each of the 256 CUs, and every further round of them
 // `round` and `more` a unit.  (Direct kernels: the unit is eight k-steps, one for each wave; tiled ones: one k-step.)  Least
-// squares over a sweep of 1 ... 8192 rows and twelve (N, K) from 320 x 320 to 10240 x 5120 and 2560 x 10240, every kernel at
-// every size; the kernel it picks is within 0.8 % of the fastest one on average and 16 % at worst.  Examples, us, 8-bit
-// activations (direct kernels by their outputs a workgroup, D, tiled ones T):
-//     48 x  5120 x 5120: D 16 x 64  7.2, D 48 x 32  8.7, D 16 x 32  8.7, T 64 x 128 15.2
-//    256 x  1280 x 1280: D 48 x 32  5.0, T 64 x 128  6.6, T 128 x 128  8.8
-//    512 x  5120 x 1280: T 64 x 128  9.3, T 128 x 128  9.5, T 256 x 256 18.3, D 64 x 32 23.4
-//   1024 x  5120 x 5120: T 128 x 256 28.9, T 128 x 128 32.3, T 64 x 128 33.2, T 256 x 256 48.8
-//   4096 x  5120 x 5120: T 128 x 128 86.9, T 256 x 256 102.6 (320 tiles: two rounds), T 64 x 128 105.7
-//   8192 x  8192 x 8192: T 256 x 256  354, T 128 x 128  439
+// squares over a sweep of 1 ... 8192 rows and fourteen (N, K) from 320 x 320 to 10240 x 5120 and 2560 x 10240, of each kernel
+// where it takes at most 1.6 times as long as the fastest; the kernel picked is within 0.7 % of the fastest one on average and
+// 23 % at worst (1024 x 1000 x 2000).  Examples, us, 8-bit activations (direct kernels by their outputs a workgroup, D, tiled
+// ones T):
+//     48 x  5120 x 5120: D 16 x 64  8.2, D 48 x 32  9.7, D 16 x 32  9.8, T 64 x 128 15.4
+//    256 x  1280 x 1280: D 48 x 32  5.3, T 64 x 128  7.1, T 128 x 128  9.2
+//    512 x  5120 x 1280: T 64 x 128  9.8, T 128 x 128 10.2, T 256 x 256 19.9, D 64 x 32 22.0
+//   1024 x  5120 x 5120: T 128 x 256 31.3, T 64 x 128 32.8, T 128 x 128 34.4, T 256 x 256 51.2
+//   4096 x  5120 x 5120: T 128 x 128 89.6, T 64 x 128 99.1, T 256 x 256 112.2 (320 tiles: two rounds)
+//   8192 x  5120 x 5120: T 256 x 256 177, T 128 x 256 179, T 128 x 128 191
 // Parts of K in several workgroups of a tiled kernel and a second launch that joins them were measured too (two and four parts)
 // and won by 6 % at most, at one size: the workgroups of a direct kernel split K among their waves already.
 enum MxKind { MX_D16x32, MX_D16x64, MX_D48x32, MX_D64x32, MX_T64x128, MX_T128x128, MX_T128x256, MX_T256x256, MX_KINDS };
 struct MxCost { int rows, cols, unit; struct { double fixed, first, round, more; } us[2]; };      // [0]: 8-bit activations, [1]: 4-bit
 static const MxCost MX_COST[MX_KINDS] = {
-    {16, 32, 8, {{3.543, 0.482, 0.376, 0.486}, {3.610, 0.376, 0.301, 0.393}}},
-    {16, 64, 8, {{3.501, 0.715, 0.704, 0.749}, {3.634, 0.576, 0.656, 0.643}}},
-    {48, 32, 8, {{3.619, 0.874, 1.461, 1.094}, {3.741, 0.566, 1.430, 0.727}}},
-    {64, 32, 8, {{3.673, 1.103, 1.782, 1.359}, {3.799, 0.694, 1.764, 0.896}}},
-    {64, 128, 1, {{4.321, 0.268, 1.492, 0.206}, {4.265, 0.266, 1.265, 0.146}}},
-    {128, 128, 1, {{4.763, 0.423, 2.150, 0.354}, {4.751, 0.323, 2.377, 0.233}}},
-    {128, 256, 1, {{5.956, 0.569, 5.441, 0.721}, {6.060, 0.457, 5.347, 0.533}}},
-    {256, 256, 1, {{7.522, 1.071, 8.450, 1.263}, {8.021, 0.658, 9.104, 0.821}}},
+    {16, 32, 8, {{3.474, 0.486, 0.250, 0.496}, {3.460, 0.397, 0.216, 0.390}}},
+    {16, 64, 8, {{3.477, 0.705, 0.645, 0.758}, {3.547, 0.569, 0.648, 0.643}}},
+    {48, 32, 8, {{3.546, 0.868, 0.790, 1.193}, {3.591, 0.585, 0.679, 0.848}}},
+    {64, 32, 8, {{3.683, 1.061, 0.816, 1.579}, {3.734, 0.705, 0.546, 1.093}}},
+    {64, 128, 1, {{4.274, 0.285, 1.169, 0.209}, {4.206, 0.268, 1.100, 0.151}}},
+    {128, 128, 1, {{4.931, 0.444, 1.975, 0.360}, {4.776, 0.338, 2.180, 0.224}}},
+    {128, 256, 1, {{6.632, 0.592, 5.571, 0.727}, {6.565, 0.456, 5.152, 0.565}}},
+    {256, 256, 1, {{10.716, 1.152, 8.790, 1.261}, {9.686, 0.678, 8.021, 0.857}}},
 };
 static_assert(MX_KINDS == SDMI_MX_ALGOS, "sdmi_mx_gemm_args.algo");
 static MxKind mx_kind(const sdmi_mx_gemm_args* a) {
@@ -625,7 +626,6 @@ template <int FMT, int MT, int NF, int KW, int U, int SRC> static int direct_lau
 }
 
 template <int FMT> static int mx_launch(const MxGemmDev& d, MxKind kind, int src, hipStream_t st) {
-    constexpr int ST = FMT == SDMI_MX_FP8 ? 3 : 4;
     // quantising: 64 columns a workgroup where 32 would make more than one for each CU (1 x 10240 x 2560: 8.4 -> 7.1 us)
     if (src >= 0 && d.N > 256 * 32) return src == 0 ? direct_launch<FMT, 1, 4, 8, 2, 0>(d, st) : src == 1 ? direct_launch<FMT, 1, 4, 8, 2, 1>(d, st) : direct_launch<FMT, 1, 4, 8, 2, 2>(d, st);
     if (src >= 0) return src == 0 ? direct_launch<FMT, 1, 2, 8, 2, 0>(d, st) : src == 1 ? direct_launch<FMT, 1, 2, 8, 2, 1>(d, st) : direct_launch<FMT, 1, 2, 8, 2, 2>(d, st);
@@ -634,10 +634,17 @@ template <int FMT> static int mx_launch(const MxGemmDev& d, MxKind kind, int src
         case MX_D16x64: return direct_launch<FMT, 1, 4, 8, 2, -1>(d, st);
         case MX_D48x32: return direct_launch<FMT, 3, 2, 8, 1, -1>(d, st);
         case MX_D64x32: return direct_launch<FMT, 4, 2, 8, 1, -1>(d, st);
-        case MX_T64x128: return tiled_launch<FMT, 64, 2, 2, 4>(d, st);
-        case MX_T128x128: return tiled_launch<FMT, 128, 2, 2, ST>(d, st);
+        // Rings no deeper than leaves room for three workgroups on a CU, whose starts and stores then run under each other's
+        // products (4096 x 10240 x 1280, 64 x 128: 8 bits 76.8 -> 69.5 us, 4 bits 62.0 -> 53.5; 128 x 128, 4 bits 48.9 -> 44.8); with
+        // 8-bit operands that is two stages of 128 x 128, which wait for their loads when they are alone on a CU
+        // (512 x 5120 x 5120, 160 tiles: 24.1 us with three stages, 29.8 with two; 4096 x 5120 x 5120, 1280 tiles: 95.7 and 90.8).
+        case MX_T64x128: return tiled_launch<FMT, 64, 2, 2, 3>(d, st);
+        case MX_T128x128:
+            if constexpr (FMT == SDMI_MX_FP8)
+                if ((d.M + 127) / 128 * ((d.N + 127) / 128) > 512) return tiled_launch<FMT, 128, 2, 2, 2>(d, st);
+            return tiled_launch<FMT, 128, 2, 2, 3>(d, st);
         case MX_T128x256: return tiled_launch<FMT, 128, 2, 4, 4>(d, st);
-        default: return tiled_launch<FMT, 256, 2, 4, ST>(d, st);
+        default: return tiled_launch<FMT, 256, 2, 4, FMT == SDMI_MX_FP8 ? 3 : 4>(d, st);      // (three 8-bit stages fill the LDS)
     }
 }
 

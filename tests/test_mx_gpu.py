@@ -286,6 +286,26 @@ def test_kernels_agree_on_large_products(dev, monkeypatch, fmt):
     assert bool(((direct - first).double().abs().cpu()[:64] <= 2 * s * ((k + 2) * 2.0 ** -23 + 7 * 2.0 ** -13)).all())
 
 
+@pytest.mark.parametrize("k", [100, 128, 200, 384, 1000, 1300])
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+def test_kernels_agree_over_many_tiles(dev, monkeypatch, fmt, k):
+    """More than 512 tiles of 128 x 128 (there 8-bit operands take a shorter ring), one k-step to eleven: every tiled kernel adds
+    in the same order, so they agree to the bit, several times over."""
+    o = ops()
+    m, n = 2990, 3010
+    q = o.mx_quantize(data(m, k, 2, "bf16", loud=False).to(dev), fmt)
+    pw = o.pack_linear_mx(torch.randn(n, k, generator=torch.Generator().manual_seed(3)).to(dev) * k ** -0.5)
+
+    def run(algo):
+        monkeypatch.setattr(o, "FORCE_MX_ALGO", algo)
+        return o.linear_mx(q, pw, out_dtype=torch.float32)
+
+    first = run(8)
+    for algo in (5, 6, 7):
+        for _ in range(4):
+            assert torch.equal(run(algo), first), algo
+
+
 @pytest.mark.parametrize("m", [1, 20, 150])
 @pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
 def test_linear_mx_picks_single_elements(dev, fmt, m):
