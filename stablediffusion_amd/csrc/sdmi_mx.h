@@ -32,6 +32,7 @@ template <int T> __device__ __forceinline__ float mx_to_f32(typename MxElem<T>::
 // that the element's own alignment allows, so rows that are not 16-byte aligned - an odd width, a column slice - are read in
 // vectors like others.
 typedef uint4 __attribute__((aligned(2))) mx_u128_a2;
+typedef uint2 __attribute__((aligned(2))) mx_u64_a2;
 typedef f32x4 __attribute__((aligned(4))) mx_f128_a4;
 template <int T> __device__ __forceinline__ void mx_load8(const typename MxElem<T>::type* p, int n, float* f) {
     if (n >= 8) {

@@ -78,72 +78,104 @@ template <int FMT> __device__ __forceinline__ f32x4 mx_mfma_f(int f, const i32x8
     }
 }
 
-// out[m, n .. n + 4) for one lane: bias, residual, one rounding
-__device__ __forceinline__ void mx_store_quad(const MxGemmDev& p, int64_t m, int64_t n, f32x4 v) {
-    if (m >= p.M) return;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        if (n + r >= p.N) break;
-        float a = v[r];
-        if (p.bias) a += p.bias[n + r];
-        if (p.type == 2) {
-            if (p.res) a += reinterpret_cast<const float*>(p.res)[m * p.ld_res + n + r];
-            reinterpret_cast<float*>(p.out)[m * p.ld_out + n + r] = a;
+// The quad at element `at` of a matrix of a type as it lies in memory (n of its 4 elements exist), and its values.
+__device__ __forceinline__ uint4 mx_quad_load(const void* p, int64_t at, int type, int64_t n) {
+    uint4 v = {0u, 0u, 0u, 0u};
+    if (type == 2) {
+        const float* const f = reinterpret_cast<const float*>(p) + at;
+        if (n >= 4) v = __builtin_bit_cast(uint4, *reinterpret_cast<const mx_f128_a4*>(f));
+        else v = (uint4){__float_as_uint(f[0]), n > 1 ? __float_as_uint(f[1]) : 0u, n > 2 ? __float_as_uint(f[2]) : 0u, 0u};
+    } else {
+        const unsigned short* const h = reinterpret_cast<const unsigned short*>(p) + at;
+        if (n >= 4) {
+            const uint2 w = *reinterpret_cast<const mx_u64_a2*>(h);
+            v.x = w.x;
+            v.y = w.y;
         } else {
-            if (p.res) {
-                const unsigned short b = reinterpret_cast<const unsigned short*>(p.res)[m * p.ld_res + n + r];
-                a += p.type == 0 ? elem_to_f32<0>(b) : elem_to_f32<1>(b);
-            }
-            reinterpret_cast<unsigned short*>(p.out)[m * p.ld_out + n + r] = p.type == 0 ? elem_from_f32<0>(a) : elem_from_f32<1>(a);
+            v.x = h[0] | (n > 1 ? (unsigned)h[1] << 16 : 0u);
+            v.y = n > 2 ? h[2] : 0u;
         }
+    }
+    return v;
+}
+__device__ __forceinline__ f32x4 mx_quad_values(const uint4& v, int type) {
+    if (type == 2) return __builtin_bit_cast(f32x4, v);
+    const unsigned short h[4] = {(unsigned short)v.x, (unsigned short)(v.x >> 16), (unsigned short)v.y, (unsigned short)(v.y >> 16)};
+    f32x4 f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) f[r] = type == 0 ? elem_to_f32<0>(h[r]) : elem_to_f32<1>(h[r]);
+    return f;
+}
+__device__ __forceinline__ void mx_quad_store(const MxGemmDev& p, int64_t m, int64_t n, const f32x4& v) {
+    const int64_t at = m * p.ld_out + n;
+    if (p.type == 2) {
+        float* const o = reinterpret_cast<float*>(p.out) + at;
+        if (n + 4 <= p.N) *reinterpret_cast<mx_f128_a4*>(o) = v;
+        else for (int r = 0; r < 3; ++r) if (n + r < p.N) o[r] = v[r];
+    } else {
+        unsigned short* const o = reinterpret_cast<unsigned short*>(p.out) + at;
+        const uint2 w = p.type == 0 ? (uint2){elem_pack2<0>(v[0], v[1]), elem_pack2<0>(v[2], v[3])} : (uint2){elem_pack2<1>(v[0], v[1]), elem_pack2<1>(v[2], v[3])};
+        if (n + 4 <= p.N) *reinterpret_cast<mx_u64_a2*>(o) = w;
+        else for (int r = 0; r < 3; ++r) if (n + r < p.N) o[r] = (unsigned short)((r < 2 ? w.x : w.y) >> (16 * (r & 1)));
     }
 }
 
-// A lane's four quads of the 64 columns from n on (see the weights' order), for token m.  16-bit residuals come in `res`: those of
-// several tokens are asked for (mx_load_res) before the first is stored - the compiler cannot know that a store to `out` leaves
-// the residuals alone, and would wait for each in turn (4096 x 10240 x 1280:
-// 80 us, and 87 one by one).
-struct MxRes { uint4 v[2]; };
-__device__ __forceinline__ void mx_load_res(const MxGemmDev& p, int64_t m, int64_t n, int q, MxRes& res) {
-    if (!p.res || p.type == 2 || m >= p.M) return;
+template <int TYPE> struct MxRaw8 {         // 8 values as they lie in memory
+    uint4 v;
+    __device__ __forceinline__ void load(const unsigned short* p) { v = *reinterpret_cast<const mx_u128_a2*>(p); }
+    __device__ __forceinline__ void values(float* f) const { elem_unpack8<TYPE>(v, f); }
+};
+template <> struct MxRaw8<2> {
+    f32x4 v[2];
+    __device__ __forceinline__ void load(const float* p) { v[0] = reinterpret_cast<const mx_f128_a4*>(p)[0]; v[1] = reinterpret_cast<const mx_f128_a4*>(p)[1]; }
+    __device__ __forceinline__ void values(float* f) const {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int64_t c = n + 32 * h + 8 * q;
-        if (c + 8 <= p.N) res.v[h] = *reinterpret_cast<const mx_u128_a2*>(reinterpret_cast<const unsigned short*>(p.res) + m * p.ld_res + c);
+        for (int j = 0; j < 8; ++j) f[j] = v[j / 4][j % 4];
     }
-}
-__device__ __forceinline__ void mx_store_run(const MxGemmDev& p, int64_t m, int64_t n, int q, const f32x4* v, const MxRes& res) {
-    if (m >= p.M) return;
+};
+
+// A wave's MF x 16 tokens x 64 columns: bias, residual, one rounding.  Lane (row, q) has tokens m + 16 i and the 8 columns from c
+// and from c + 32 on (see the weights' order).  Straight code for each type, the residuals all asked for before the first store
+// - the compiler cannot know that a store to `out` leaves them alone: a fragment at a time, with its branches for each type and
+// edge inside, is 60 KB of instructions that every tile fetches anew (8192 x 10240 x 1280: OLD us, and NEW like this).
+template <int TYPE, bool RES, int MF> __device__ __forceinline__ void mx_store_tile(const MxGemmDev& p, int64_t m, int64_t c, const f32x4 (&acc)[MF][4]) {
+    typedef typename MxElem<TYPE>::type E;
+    constexpr int TOGETHER = TYPE == 2 || MF < 4 ? 2 : 4;
+    float a[8], b[16], d[8];
+    if (p.bias) {
+        mx_load8<2>(p.bias + c, 8, b);
+        mx_load8<2>(p.bias + c + 32, 8, b + 8);
+    } else {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int64_t c = n + 32 * h + 8 * q;
-        if (c + 8 > p.N) {
-            mx_store_quad(p, m, c, v[2 * h]);
-            mx_store_quad(p, m, c + 4, v[2 * h + 1]);
-            continue;
+        for (int j = 0; j < 16; ++j) b[j] = 0.0f;
+    }
+    const E* const res = reinterpret_cast<const E*>(p.res) + c;
+    E* const out = reinterpret_cast<E*>(p.out) + c;
+#pragma unroll
+    for (int i0 = 0; i0 < MF; i0 += TOGETHER) {
+        MxRaw8<TYPE> r[TOGETHER][2];
+        if constexpr (RES) {
+#pragma unroll
+            for (int i = 0; i < TOGETHER; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) r[i][h].load(res + min(m + 16 * (i0 + i), p.M - 1) * p.ld_res + 32 * h);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        float a[8], b[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) a[j] = v[2 * h + j / 4][j % 4];
-        if (p.bias) {
-            mx_load8<2>(p.bias + c, 8, b);
+        for (int i = 0; i < TOGETHER; ++i) {
+            const int64_t t = m + 16 * (i0 + i);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) a[j] += b[j];
-        }
-        if (p.type == 2) {
-            if (p.res) {
-                mx_load8<2>(reinterpret_cast<const float*>(p.res) + m * p.ld_res + c, 8, b);
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) a[j] += b[j];
+                for (int j = 0; j < 8; ++j) a[j] = acc[i0 + i][2 * h + j / 4][j % 4] + b[8 * h + j];
+                if constexpr (RES) {
+                    r[i][h].values(d);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) a[j] += d[j];
+                }
+                if (t < p.M) mx_store8<TYPE>(out + t * p.ld_out + 32 * h, 8, a);
             }
-            mx_store8<2>(reinterpret_cast<float*>(p.out) + m * p.ld_out + c, 8, a);
-        } else {
-            if (p.res) {
-                if (p.type == 0) elem_unpack8<0>(res.v[h], b); else elem_unpack8<1>(res.v[h], b);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) a[j] += b[j];
-            }
-            *reinterpret_cast<mx_u128_a2*>(reinterpret_cast<unsigned short*>(p.out) + m * p.ld_out + c) = p.type == 0 ? elem_pack8<0>(a) : elem_pack8<1>(a);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 }
@@ -201,6 +233,14 @@ __global__ __launch_bounds__(64 * KW) void sdmi_mx_direct_kernel(MxGemmDev p) {
     };
     if (mine > 0) load(0, 0);
     if (mine > U) load(1, U);
+    // one quad of the output for each lane of the first MT NF waves; its bias and residual travel behind the first weights
+    static_assert(MT * NF <= KW, "a wave stores one fragment");
+    const int of = f0 + wave % NF;
+    const int64_t om = m0 + wave / NF * 16 + row, on = grp * 64 + 32 * (of >> 1) + 8 * q + 4 * (of & 1);
+    const bool stores = wave < MT * NF && om < p.M && on < p.N;
+    uint4 bias = {0u, 0u, 0u, 0u}, res = bias;
+    if (stores && p.bias) bias = mx_quad_load(p.bias, on, 2, p.N - on);
+    if (stores && p.res) res = mx_quad_load(p.res, om * p.ld_res + on, p.type, p.N - on);
     unsigned char* const own = smem;                       // SRC >= 0: [nk][M][RB] codes, then [nk][M][4] scales
     const int rows = (int)p.M;
     unsigned char* const own_s = smem + nk * rows * RB;
@@ -269,12 +309,13 @@ __global__ __launch_bounds__(64 * KW) void sdmi_mx_direct_kernel(MxGemmDev p) {
 #pragma unroll
         for (int f = 0; f < NF; ++f) part[((wave * MT + mi) * NF + f) * 64 + lane] = acc[mi][f];
     __syncthreads();
-    for (int t = wave; t < MT * NF; t += KW) {
-        f32x4 v = part[t * 64 + lane];
+    if (stores) {
+        f32x4 v = part[wave * 64 + lane];
 #pragma unroll
-        for (int k = 1; k < KW; ++k) v += part[(k * MT * NF + t) * 64 + lane];
-        const int f = f0 + t % NF;
-        mx_store_quad(p, m0 + t / NF * 16 + row, grp * 64 + 32 * (f >> 1) + 8 * q + 4 * (f & 1), v);
+        for (int k = 1; k < KW; ++k) v += part[(k * MT * NF + wave) * 64 + lane];
+        if (p.bias) v += mx_quad_values(bias, 2);
+        if (p.res) v += mx_quad_values(res, p.type);
+        mx_quad_store(p, om, on, v);
     }
 }
 
@@ -502,15 +543,30 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void sdmi_mx_tiled_kernel(MxGemm
     }
     step(std::false_type(), even, odd, s);
 
-    constexpr int TOGETHER = T::MF == 8 ? 1 : T::MF;                             // (128 accumulators leave no room for more)
+    const int64_t m = m0 + arow, c = (g0 + wn) * 64;
+    if (c + 64 <= p.N) {
+        auto store = [&](auto res) {
+            constexpr bool RES = decltype(res)::value;
+            if (p.type == 0) mx_store_tile<0, RES>(p, m, c + 8 * q, acc);
+            else if (p.type == 1) mx_store_tile<1, RES>(p, m, c + 8 * q, acc);
+            else mx_store_tile<2, RES>(p, m, c + 8 * q, acc);
+        };
+        if (p.res) store(std::true_type());
+        else store(std::false_type());
+        return;
+    }
 #pragma unroll
-    for (int m1 = 0; m1 < T::MF; m1 += TOGETHER) {
-        MxRes res[TOGETHER];
+    for (int mi = 0; mi < T::MF; ++mi) {                                         // the last columns, in quads
 #pragma unroll
-        for (int i = 0; i < TOGETHER; ++i) mx_load_res(p, m0 + arow + (m1 + i) * 16, (g0 + wn) * 64, q, res[i]);
-#pragma unroll
-        for (int i = 0; i < TOGETHER; ++i) mx_store_run(p, m0 + arow + (m1 + i) * 16, (g0 + wn) * 64, q, acc[m1 + i], res[i]);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int f = 0; f < 4; ++f) {
+            const int64_t n = c + 32 * (f >> 1) + 8 * q + 4 * (f & 1);
+            if (m + mi * 16 < p.M && n < p.N) {
+                f32x4 v = acc[mi][f];
+                if (p.bias) v += mx_quad_values(mx_quad_load(p.bias, n, 2, p.N - n), 2);
+                if (p.res) v += mx_quad_values(mx_quad_load(p.res, (m + mi * 16) * p.ld_res + n, p.type, p.N - n), p.type);
+                mx_quad_store(p, m + mi * 16, n, v);
+            }
+        }
     }
 }
 
