@@ -120,60 +120,102 @@ __device__ __forceinline__ void mx_quad_store(const MxGemmDev& p, int64_t m, int
     }
 }
 
-template <int TYPE> struct MxRaw8 {         // 8 values as they lie in memory
-    uint4 v;
-    __device__ __forceinline__ void load(const unsigned short* p) { v = *reinterpret_cast<const mx_u128_a2*>(p); }
-    __device__ __forceinline__ void values(float* f) const { elem_unpack8<TYPE>(v, f); }
-};
-template <> struct MxRaw8<2> {
-    f32x4 v[2];
-    __device__ __forceinline__ void load(const float* p) { v[0] = reinterpret_cast<const mx_f128_a4*>(p)[0]; v[1] = reinterpret_cast<const mx_f128_a4*>(p)[1]; }
-    __device__ __forceinline__ void values(float* f) const {
+// Stores and residual loads of whole lines.  A lane of the accumulators has 16-byte pieces of one token; stored as they lie, the 64
+// lanes' addresses are 64 to a kilobyte of output, and each instruction writes parts of lines.  Pairs of pieces are therefore
+// passed between lanes so that lane l holds piece l % 8 of one 128-byte line of token l / 8, in the first of the two for tokens
+// 0 ... 7 of a fragment and in the second for 8 ... 15.  (8-bit pieces of a pair: columns c and c + 32 of 16-bit types, 4 and 4 of fp32.)
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 __attribute__((aligned(2))) mx_u32x4_a2;
+__device__ __forceinline__ void mx_swap_rows(u32x4& a, u32x4& b, bool upper) {       // rows 0 - 7's b for rows 8 - 15's a; its own inverse
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = v[j / 4][j % 4];
+    for (int j = 0; j < 4; ++j) {
+        const unsigned got = __builtin_amdgcn_update_dpp(0, upper ? a[j] : b[j], 0x128, 0xf, 0xf, true);     // row_ror:8
+        a[j] = upper ? got : a[j];
+        b[j] = upper ? b[j] : got;
     }
-};
+}
+__device__ __forceinline__ void mx_permute(u32x4& a, int from) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] = __builtin_amdgcn_ds_bpermute(from, a[j]);
+}
 
-// A wave's MF x 16 tokens x 64 columns: bias, residual, one rounding.  Lane (row, q) has tokens m + 16 i and the 8 columns from c
-// and from c + 32 on (see the weights' order).  Straight code for each type, the residuals all asked for before the first store
-// - the compiler cannot know that a store to `out` leaves them alone: a fragment at a time, with its branches for each type and
-// edge inside, is 60 KB of instructions that every tile fetches anew (8192 x 10240 x 1280: OLD us, and NEW like this).
-template <int TYPE, bool RES, int MF> __device__ __forceinline__ void mx_store_tile(const MxGemmDev& p, int64_t m, int64_t c, const f32x4 (&acc)[MF][4]) {
+// A wave's MF x 16 tokens (from m on) x 64 columns (from c on): bias, residual, one rounding.  Straight code for each type, the
+// residuals of several fragments asked for before the first of them is stored - the compiler cannot know that a store to `out`
+// leaves them alone.
+template <int TYPE, bool RES, int MF> __device__ __forceinline__ void mx_store_tile(const MxGemmDev& p, int64_t m, int64_t c, int lane, const f32x4 (&acc)[MF][4]) {
     typedef typename MxElem<TYPE>::type E;
-    constexpr int TOGETHER = TYPE == 2 || MF < 4 ? 2 : 4;
-    float a[8], b[16], d[8];
+    constexpr int PAIRS = TYPE == 2 ? 2 : 1, PIECE = 16 / (int)sizeof(E), TOGETHER = TYPE == 2 || MF < 4 ? 2 : 4;
+    const int row = lane & 15, q = lane >> 4, t8 = lane >> 3, c8 = lane & 7;
+    const bool upper = row & 8;
+    const int there = 4 * (TYPE == 2 ? t8 + 8 * (c8 & 1) + 16 * (c8 >> 1) : t8 + 8 * (c8 >> 2) + 16 * (c8 & 3));
+    const int back = 4 * (8 * (row & 7) + (TYPE == 2 ? 2 * q + (row >> 3) : q + 4 * (row >> 3)));
+    float b[16];
     if (p.bias) {
-        mx_load8<2>(p.bias + c, 8, b);
-        mx_load8<2>(p.bias + c + 32, 8, b + 8);
+        mx_load8<2>(p.bias + c + 8 * q, 8, b);
+        mx_load8<2>(p.bias + c + 8 * q + 32, 8, b + 8);
     } else {
 #pragma unroll
         for (int j = 0; j < 16; ++j) b[j] = 0.0f;
     }
-    const E* const res = reinterpret_cast<const E*>(p.res) + c;
-    E* const out = reinterpret_cast<E*>(p.out) + c;
+    const E* const res = reinterpret_cast<const E*>(p.res) + c + c8 * PIECE;
+    E* const out = reinterpret_cast<E*>(p.out) + c + c8 * PIECE;
 #pragma unroll
     for (int i0 = 0; i0 < MF; i0 += TOGETHER) {
-        MxRaw8<TYPE> r[TOGETHER][2];
+        u32x4 r[TOGETHER][PAIRS][2];
         if constexpr (RES) {
 #pragma unroll
             for (int i = 0; i < TOGETHER; ++i)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) r[i][h].load(res + min(m + 16 * (i0 + i), p.M - 1) * p.ld_res + 32 * h);
+                for (int h = 0; h < PAIRS; ++h)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        r[i][h][k] = __builtin_nontemporal_load(reinterpret_cast<const mx_u32x4_a2*>(res + min(m + 16 * (i0 + i) + 8 * k + t8, p.M - 1) * p.ld_res + 32 * h));
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int i = 0; i < TOGETHER; ++i) {
-            const int64_t t = m + 16 * (i0 + i);
+            float a[16];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int j = 0; j < 16; ++j) a[j] = acc[i0 + i][j / 4][j % 4] + b[j];
+            if constexpr (RES) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) a[j] = acc[i0 + i][2 * h + j / 4][j % 4] + b[8 * h + j];
-                if constexpr (RES) {
-                    r[i][h].values(d);
+                for (int h = 0; h < PAIRS; ++h) {
+                    mx_permute(r[i][h][0], back);
+                    mx_permute(r[i][h][1], back);
+                    mx_swap_rows(r[i][h][0], r[i][h][1], upper);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) a[j] += d[j];
+                    for (int k = 0; k < 2; ++k) {
+                        float d[8];
+                        if constexpr (TYPE == 2) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) d[j] = __uint_as_float(r[i][h][k][j]);
+                        } else {
+                            elem_unpack8<TYPE>(__builtin_bit_cast(uint4, r[i][h][k]), d);
+                        }
+#pragma unroll
+                        for (int j = 0; j < PIECE; ++j) a[8 * h + PIECE * k + j] += d[j];
+                    }
                 }
-                if (t < p.M) mx_store8<TYPE>(out + t * p.ld_out + 32 * h, 8, a);
+            }
+#pragma unroll
+            for (int h = 0; h < PAIRS; ++h) {
+                u32x4 v[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    if constexpr (TYPE == 2) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[k][j] = __float_as_uint(a[8 * h + 4 * k + j]);
+                    } else {
+                        v[k] = __builtin_bit_cast(u32x4, elem_pack8<TYPE>(a + 8 * k));
+                    }
+                }
+                mx_swap_rows(v[0], v[1], upper);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    mx_permute(v[k], there);
+                    const int64_t t = m + 16 * (i0 + i) + 8 * k + t8;
+                    if (t < p.M) __builtin_nontemporal_store(v[k], reinterpret_cast<mx_u32x4_a2*>(out + t * p.ld_out + 32 * h));
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -547,9 +589,9 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void sdmi_mx_tiled_kernel(MxGemm
     if (c + 64 <= p.N) {
         auto store = [&](auto res) {
             constexpr bool RES = decltype(res)::value;
-            if (p.type == 0) mx_store_tile<0, RES>(p, m, c + 8 * q, acc);
-            else if (p.type == 1) mx_store_tile<1, RES>(p, m, c + 8 * q, acc);
-            else mx_store_tile<2, RES>(p, m, c + 8 * q, acc);
+            if (p.type == 0) mx_store_tile<0, RES>(p, m0 + wm * T::MF * 16, c, lane, acc);
+            else if (p.type == 1) mx_store_tile<1, RES>(p, m0 + wm * T::MF * 16, c, lane, acc);
+            else mx_store_tile<2, RES>(p, m0 + wm * T::MF * 16, c, lane, acc);
         };
         if (p.res) store(std::true_type());
         else store(std::false_type());
