@@ -120,10 +120,13 @@ __device__ __forceinline__ void mx_quad_store(const MxGemmDev& p, int64_t m, int
     }
 }
 
-// Stores and residual loads of whole lines.  A lane of the accumulators has 16-byte pieces of one token; stored as they lie, the 64
-// lanes' addresses are 64 to a kilobyte of output, and each instruction writes parts of lines.  Pairs of pieces are therefore
-// passed between lanes so that lane l holds piece l % 8 of one 128-byte line of token l / 8, in the first of the two for tokens
-// 0 ... 7 of a fragment and in the second for 8 ... 15.  (8-bit pieces of a pair: columns c and c + 32 of 16-bit types, 4 and 4 of fp32.)
+// Stores and residual loads of whole lines.  A lane of the accumulators has 16-byte pieces of one token, and neighbouring lanes
+// are neighbouring TOKENS: stored as they lie, a kilobyte of output is 64 addresses in 16 half lines.  So pairs of pieces (of
+// 16-bit types columns c and c + 32, of fp32 c and c + 4) go round the lanes until lane l holds piece l % 8 of a 128-byte line of
+// token l / 8, in the first of the two for tokens 0 ... 7 of the fragment and in the second for 8 ... 15; residuals take the same
+// way back.  (8192 x 10240 x 1280, 256 x 256 tiles, us: 4 bits 90 -> 86, with residual 121 -> 117; 4096 x 10240 x 1280 fp32
+// 86 -> 79.  Stores past the caches were faster by themselves, 72 for 86, but whatever reads the output next then fetches it from memory:
+// 8192 x 10240 x 5120 with the quantisation of its output 235 us, and 243 like that.)
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 __attribute__((aligned(2))) mx_u32x4_a2;
 __device__ __forceinline__ void mx_swap_rows(u32x4& a, u32x4& b, bool upper) {       // rows 0 - 7's b for rows 8 - 15's a; its own inverse
@@ -169,7 +172,7 @@ template <int TYPE, bool RES, int MF> __device__ __forceinline__ void mx_store_t
                 for (int h = 0; h < PAIRS; ++h)
 #pragma unroll
                     for (int k = 0; k < 2; ++k)
-                        r[i][h][k] = __builtin_nontemporal_load(reinterpret_cast<const mx_u32x4_a2*>(res + min(m + 16 * (i0 + i) + 8 * k + t8, p.M - 1) * p.ld_res + 32 * h));
+                        r[i][h][k] = *reinterpret_cast<const mx_u32x4_a2*>(res + min(m + 16 * (i0 + i) + 8 * k + t8, p.M - 1) * p.ld_res + 32 * h);
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
@@ -214,7 +217,7 @@ template <int TYPE, bool RES, int MF> __device__ __forceinline__ void mx_store_t
                 for (int k = 0; k < 2; ++k) {
                     mx_permute(v[k], there);
                     const int64_t t = m + 16 * (i0 + i) + 8 * k + t8;
-                    if (t < p.M) __builtin_nontemporal_store(v[k], reinterpret_cast<mx_u32x4_a2*>(out + t * p.ld_out + 32 * h));
+                    if (t < p.M) *reinterpret_cast<mx_u32x4_a2*>(out + t * p.ld_out + 32 * h) = v[k];
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -646,28 +649,28 @@ static bool mx_args_ok(const sdmi_mx_gemm_args* a) {
 // launch costs `fixed` us, a unit of K `first` for the first workgroup on each of the 256 CUs, and every further round of them
 // `round` and `more` a unit.  (Direct kernels: the unit is eight k-steps, one for each wave; tiled ones: one k-step.)  Least
 // squares over a sweep of 1 ... 8192 rows and fourteen (N, K) from 320 x 320 to 10240 x 5120 and 2560 x 10240, of each kernel
-// where it takes at most 1.6 times as long as the fastest; the kernel picked is within 0.7 % of the fastest one on average and
-// 23 % at worst (1024 x 1000 x 2000).  Examples, us, 8-bit activations (direct kernels by their outputs a workgroup, D, tiled
+// where it takes at most twice as long as the fastest; the kernel picked is within 1 % of the fastest one on average and 24 % at
+// worst (1 x 1280 x 1280, a microsecond).  Examples, us, 8-bit activations (direct kernels by their outputs a workgroup, D, tiled
 // ones T):
-//     48 x  5120 x 5120: D 16 x 64  8.2, D 48 x 32  9.7, D 16 x 32  9.8, T 64 x 128 15.4
-//    256 x  1280 x 1280: D 48 x 32  5.3, T 64 x 128  7.1, T 128 x 128  9.2
-//    512 x  5120 x 1280: T 64 x 128  9.8, T 128 x 128 10.2, T 256 x 256 19.9, D 64 x 32 22.0
-//   1024 x  5120 x 5120: T 128 x 256 31.3, T 64 x 128 32.8, T 128 x 128 34.4, T 256 x 256 51.2
-//   4096 x  5120 x 5120: T 128 x 128 89.6, T 64 x 128 99.1, T 256 x 256 112.2 (320 tiles: two rounds)
-//   8192 x  5120 x 5120: T 256 x 256 177, T 128 x 256 179, T 128 x 128 191
+//     48 x  5120 x 5120: D 16 x 64  7.6, D 48 x 32  9.2, D 16 x 32  9.2, T 64 x 128 15.1
+//    256 x  1280 x 1280: D 48 x 32  5.0, T 64 x 128  6.6, T 128 x 128  8.5
+//    512 x  5120 x 1280: T 128 x 128  9.4, T 64 x 128  9.4, T 256 x 256 17.0, D 64 x 32 18.6
+//   1024 x  5120 x 5120: T 64 x 128 30.6, T 128 x 256 31.6, T 128 x 128 33.4, T 256 x 256 47.9
+//   4096 x  5120 x 5120: T 128 x 128 85.1, T 64 x 128 96.8, T 256 x 256 102.9 (320 tiles: two rounds)
+//   8192 x  5120 x 5120: T 256 x 256 171, T 128 x 256 177, T 128 x 128 190
 // Parts of K in several workgroups of a tiled kernel and a second launch that joins them were measured too (two and four parts)
 // and won by 6 % at most, at one size: the workgroups of a direct kernel split K among their waves already.
 enum MxKind { MX_D16x32, MX_D16x64, MX_D48x32, MX_D64x32, MX_T64x128, MX_T128x128, MX_T128x256, MX_T256x256, MX_KINDS };
 struct MxCost { int rows, cols, unit; struct { double fixed, first, round, more; } us[2]; };      // [0]: 8-bit activations, [1]: 4-bit
 static const MxCost MX_COST[MX_KINDS] = {
-    {16, 32, 8, {{3.474, 0.486, 0.250, 0.496}, {3.460, 0.397, 0.216, 0.390}}},
-    {16, 64, 8, {{3.477, 0.705, 0.645, 0.758}, {3.547, 0.569, 0.648, 0.643}}},
-    {48, 32, 8, {{3.546, 0.868, 0.790, 1.193}, {3.591, 0.585, 0.679, 0.848}}},
-    {64, 32, 8, {{3.683, 1.061, 0.816, 1.579}, {3.734, 0.705, 0.546, 1.093}}},
-    {64, 128, 1, {{4.274, 0.285, 1.169, 0.209}, {4.206, 0.268, 1.100, 0.151}}},
-    {128, 128, 1, {{4.931, 0.444, 1.975, 0.360}, {4.776, 0.338, 2.180, 0.224}}},
-    {128, 256, 1, {{6.632, 0.592, 5.571, 0.727}, {6.565, 0.456, 5.152, 0.565}}},
-    {256, 256, 1, {{10.716, 1.152, 8.790, 1.261}, {9.686, 0.678, 8.021, 0.857}}},
+    {16, 32, 8, {{3.542, 0.412, 0.157, 0.480}, {3.537, 0.340, 0.214, 0.345}}},
+    {16, 64, 8, {{3.449, 0.624, 0.482, 0.716}, {3.514, 0.528, 0.492, 0.567}}},
+    {48, 32, 8, {{3.440, 0.820, 0.596, 1.134}, {3.554, 0.519, 0.537, 0.791}}},
+    {64, 32, 8, {{3.377, 1.059, 0.544, 1.449}, {3.506, 0.681, 0.736, 0.997}}},
+    {64, 128, 1, {{4.086, 0.278, 0.939, 0.200}, {4.048, 0.257, 0.929, 0.147}}},
+    {128, 128, 1, {{4.530, 0.426, 1.462, 0.360}, {4.415, 0.331, 1.710, 0.220}}},
+    {128, 256, 1, {{5.473, 0.610, 4.259, 0.748}, {5.428, 0.452, 4.360, 0.541}}},
+    {256, 256, 1, {{6.915, 1.100, 6.615, 1.250}, {6.885, 0.647, 6.995, 0.833}}},
 };
 static_assert(MX_KINDS == SDMI_MX_ALGOS, "sdmi_mx_gemm_args.algo");
 static MxKind mx_kind(const sdmi_mx_gemm_args* a) {
