@@ -468,7 +468,7 @@ typedef struct sdmi_mx_gemm_args {
     const void* w_codes;
     const void* w_scales;
     const float* bias;       /* [N] or NULL */
-    const void* res;         /* [M, N] of out_dtype or NULL */
+    const void* res;         /* [M, N] of out_dtype or NULL; may be out itself, with ld_res = ld_out */
     void* out;               /* [M, N] of out_dtype */
     void* workspace;         /* sdmi_mx_gemm_workspace_bytes(args) bytes; NULL where that is 0 */
     int64_t workspace_bytes;

@@ -1,5 +1,7 @@
 """The block-scaled (MX) operators against plain 64-bit statements of the same operators (mx_oracle): quantisation exactly,
 everything else to bounds that are derived where they stand."""
+import ctypes
+
 import pytest
 import torch
 
@@ -304,6 +306,41 @@ def test_kernels_agree_over_many_tiles(dev, monkeypatch, fmt, k):
     for algo in (5, 6, 7):
         for _ in range(4):
             assert torch.equal(run(algo), first), algo
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("algo", range(1, 9))
+def test_every_kernel_adds_and_rounds_once(dev, monkeypatch, algo, dtype):
+    """Bias and residual of every type, added in fp32 and rounded once: bit for bit what the kernel's own fp32 products give.
+    Rows and columns that end inside a tile, a column group and a quad, residuals of any stride, outputs in place of the residual."""
+    from stablediffusion_amd import hip
+    o = ops()
+    monkeypatch.setattr(o, "FORCE_MX_ALGO", algo)
+    t = TYPES[dtype]
+    for i, (m, n) in enumerate([(1, 64), (15, 66), (130, 128), (260, 323), (400, 576), (257, 1)]):
+        k = 150 + 128 * i
+        g = torch.Generator().manual_seed(300 + i)
+        w, bias, res = torch.randn(n, k, generator=g) * k ** -0.5, torch.randn(n, generator=g).to(dev), torch.randn(m, n, generator=g).to(t)
+        q = o.mx_quantize(data(m, k, i, "bf16", loud=False).to(dev), ["mxfp8", "mxfp4"][i % 2])
+        bare, with_bias = o.pack_linear_mx(w.to(dev)), o.pack_linear_mx(w.to(dev), bias)
+        sums = o.linear_mx(q, bare, out_dtype=torch.float32)
+        for pad in (0, 1, 8):
+            r = strided(res, dev, pad)
+            assert torch.equal(o.linear_mx(q, bare, res=r), (sums + r.float()).to(t)), (m, n, pad)
+            assert torch.equal(o.linear_mx(q, with_bias, res=r), (sums + bias + r.float()).to(t)), (m, n, pad)
+            assert torch.equal(o.linear_mx(q, with_bias, out_dtype=t), (sums + bias).to(t)), (m, n, pad)
+            # in place of the residual, a column slice of a buffer whose other columns stay as they were
+            wide = torch.full((m, n + 2 * pad), 7.0, dtype=t, device=dev)
+            own = wide[:, pad:pad + n]
+            own.copy_(r)
+            a = hip.MxGemmArgs()
+            a.x_codes, a.x_scales, a.fmt = q.codes_ptr, q.scales_ptr, [hip.MX_FP8, hip.MX_FP4][i % 2]
+            a.w_codes, a.w_scales, a.bias = with_bias.codes_ptr, with_bias.scales_ptr, with_bias.bias_ptr
+            a.M, a.N, a.K, a.out, a.res, a.ld_out, a.ld_res = m, n, k, own.data_ptr(), own.data_ptr(), own.stride(0), own.stride(0)
+            a.out_dtype, a.algo = o._mx_dt(t, "test"), algo
+            hip.check(hip.lib().sdmi_mx_gemm(ctypes.byref(a), torch.cuda.current_stream().cuda_stream), "sdmi_mx_gemm")
+            assert torch.equal(own, (sums + bias + r.float()).to(t)), (m, n, pad)
+            assert bool((wide[:, :pad] == 7.0).all()) and bool((wide[:, pad + n:] == 7.0).all()), (m, n, pad)
 
 
 @pytest.mark.parametrize("m", [1, 20, 150])
