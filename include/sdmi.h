@@ -460,7 +460,7 @@ int sdmi_mx_pack_linear(const void* w, int64_t ldw, int64_t N, int64_t K, int32_
                         void* stream);
 
 /* out[m, n] = sum_k x[m, k] w[n, k] + bias[n] + res[m, n]: block-scaled operands, fp32 accumulation in an order that
- * depends on the sizes alone, one rounding to out_dtype. */
+ * depends on the sizes and on whether x comes quantised, one rounding to out_dtype. */
 typedef struct sdmi_mx_gemm_args {
     const void* x;           /* [M, K] of x_dtype, quantised to fmt on the way, or NULL: x_codes / x_scales hold it */
     const void* x_codes;

@@ -225,13 +225,28 @@ template <int TYPE, bool RES, int MF> __device__ __forceinline__ void mx_store_t
     }
 }
 
+template <int T> struct MxRaw8 {             // 8 values as they lie in memory
+    uint4 v;
+    __device__ __forceinline__ void load(const unsigned short* p) { v = *reinterpret_cast<const mx_u128_a2*>(p); }
+    __device__ __forceinline__ void clear() { v = (uint4){0u, 0u, 0u, 0u}; }
+    __device__ __forceinline__ void values(float* f) const { elem_unpack8<T>(v, f); }
+};
+template <> struct MxRaw8<2> {
+    f32x4 v[2];
+    __device__ __forceinline__ void load(const float* p) { v[0] = reinterpret_cast<const mx_f128_a4*>(p)[0]; v[1] = reinterpret_cast<const mx_f128_a4*>(p)[1]; }
+    __device__ __forceinline__ void clear() { v[0] = v[1] = (f32x4){0.f, 0.f, 0.f, 0.f}; }
+    __device__ __forceinline__ void values(float* f) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = v[j / 4][j % 4];
+    }
+};
+
 // ---- direct form --------------------------------------------------------------------------------------------------------
 // Few tokens: the weights' bytes are the work, and a workgroup has to have many of them in flight.  It takes NF of a group's
 // four fragments for MT x 16 tokens; its KW waves take every KW-th k-step from memory straight into
 // registers, U k-steps ahead of the ones they multiply, and join their sums through LDS in a fixed order.
-// SRC >= 0: x is a plain matrix of that type (mx_src_type) and few rows (mx_fused), which every workgroup quantises for itself
+// SRC >= 0: x is a plain matrix of that type (mx_src_type), of which every workgroup quantises its rows for itself (mx_fused),
 // into LDS while its first weights are on their way: one launch instead of two.
-constexpr int MX_FUSED_PAIRS = 16;        // (k-step, row) pairs that a wave quantises: what its lanes load in one go
 
 template <int FMT, int MT, int NF, int KW, int U, int SRC>
 __global__ __launch_bounds__(64 * KW) void sdmi_mx_direct_kernel(MxGemmDev p) {
@@ -286,29 +301,33 @@ __global__ __launch_bounds__(64 * KW) void sdmi_mx_direct_kernel(MxGemmDev p) {
     uint4 bias = {0u, 0u, 0u, 0u}, res = bias;
     if (stores && p.bias) bias = mx_quad_load(p.bias, on, 2, p.N - on);
     if (stores && p.res) res = mx_quad_load(p.res, om * p.ld_res + on, p.type, p.N - on);
-    unsigned char* const own = smem;                       // SRC >= 0: [nk][M][RB] codes, then [nk][M][4] scales
-    const int rows = (int)p.M;
+    unsigned char* const own = smem;                       // SRC >= 0: [nk][rows][RB] codes, then [nk][rows][4] scales
+    const int rows = (int)min(p.M - m0, (int64_t)(16 * MT));
     unsigned char* const own_s = smem + nk * rows * RB;
     if constexpr (SRC >= 0) {
-        // the wave quantises the k-steps that it alone will read: four (k-step, row) pairs at a time, 16 lanes each, and AT
-        // times four on their way together (pairs past the end: the last one again)
-        constexpr int AT = MX_FUSED_PAIRS / 4;
-        const typename MxElem<SRC>::type* const x = reinterpret_cast<const typename MxElem<SRC>::type*>(p.x);
-        const int pairs = mine * rows;
-        if (pairs > 0) {
-            float f[AT][8];
+        // the wave quantises the k-steps that it alone will read: four (k-step, row) pairs at a time, 16 lanes each, and the
+        // 16 MT rows of a k-step on their way together (rows and pairs past the end: the last one again)
+        typedef typename MxElem<SRC>::type E;
+        constexpr int AT = 4 * MT;
+        const E* const x = reinterpret_cast<const E*>(p.x) + m0 * p.ldx;
+        const int sh = rows > 1 ? 32 - __builtin_clz(rows - 1) : 0, pairs = mine << sh;          // (rows rounded up to a power of two)
+        for (int j0 = 0; j0 < pairs; j0 += 4 * AT) {
+            MxRaw8<SRC> raw[AT];
             int at[AT];
 #pragma unroll
             for (int u = 0; u < AT; ++u) {
-                const int j = min(4 * u + q, pairs - 1), step = wave + (j / rows) * KW, r = j % rows;
+                const int j = min(j0 + 4 * u + q, pairs - 1), step = wave + (j >> sh) * KW, r = min(j & ((1 << sh) - 1), rows - 1);
                 const int64_t k0 = (int64_t)step * MX_KSTEP + row * 8;
                 at[u] = step * rows + r;
-                mx_load8<SRC>(x + r * p.ldx + k0, (int)max((int64_t)0, min((int64_t)8, p.K - k0)), f[u]);
+                raw[u].load(x + r * p.ldx + min(k0, p.K - 8));                   // (K is whole eights: mx_fused)
+                if (k0 >= p.K) raw[u].clear();
             }
 #pragma unroll
             for (int u = 0; u < AT; ++u) {
+                float f[8];
+                raw[u].values(f);
                 uint2 c;
-                const unsigned dw = mx_quantise8<FMT>(f[u], lane, c);
+                const unsigned dw = mx_quantise8<FMT>(f, lane, c);
                 if constexpr (FMT == SDMI_MX_FP8) *reinterpret_cast<uint2*>(own + at[u] * RB + row * 8) = c;
                 else *reinterpret_cast<unsigned*>(own + at[u] * RB + row * 4) = c.x;
                 if (row == 0) *reinterpret_cast<unsigned*>(own_s + at[u] * 4) = dw;
@@ -329,7 +348,7 @@ __global__ __launch_bounds__(64 * KW) void sdmi_mx_direct_kernel(MxGemmDev p) {
                     else x = mx_op4(a[buf][u][mi]);
                     sc = xsc[buf][u][mi];
                 } else {
-                    const int at = (wave + (i0 + u) * KW) * rows + min(row, rows - 1);
+                    const int at = (wave + (i0 + u) * KW) * rows + min(mi * 16 + row, rows - 1);
                     const uint4 lo = *reinterpret_cast<const uint4*>(own + at * RB + q * 16);
                     if constexpr (FMT == SDMI_MX_FP8) x = mx_op8(lo, *reinterpret_cast<const uint4*>(own + at * RB + q * 16 + 64));
                     else x = mx_op4(lo);
@@ -673,27 +692,46 @@ static const MxCost MX_COST[MX_KINDS] = {
     {256, 256, 1, {{6.915, 1.100, 6.615, 1.250}, {6.885, 0.647, 6.995, 0.833}}},
 };
 static_assert(MX_KINDS == SDMI_MX_ALGOS, "sdmi_mx_gemm_args.algo");
+static int64_t mx_rounds(const sdmi_mx_gemm_args* a, int kind) {
+    const MxCost& c = MX_COST[kind];
+    return ((a->M + c.rows - 1) / c.rows * ((a->N + c.cols - 1) / c.cols) + 255) / 256;
+}
+static double mx_cost(const sdmi_mx_gemm_args* a, int kind) {
+    const MxCost& c = MX_COST[kind];
+    const auto& us = c.us[a->fmt == SDMI_MX_FP8 ? 0 : 1];
+    const double units = (double)((mx_ksteps(a->K) + c.unit - 1) / c.unit);
+    return us.fixed + us.first * units + (double)(mx_rounds(a, kind) - 1) * (us.round + us.more * units);
+}
 static MxKind mx_kind(const sdmi_mx_gemm_args* a) {
     if (a->algo) return (MxKind)(a->algo - 1);
-    const int b = a->fmt == SDMI_MX_FP8 ? 0 : 1;
     int best = MX_T256x256;
-    double least = 0;
-    for (int i = MX_KINDS - 1; i >= 0; --i) {
-        const MxCost& c = MX_COST[i];
-        const int64_t blocks = (a->M + c.rows - 1) / c.rows * ((a->N + c.cols - 1) / c.cols), rounds = (blocks + 255) / 256;
-        const double units = (double)((mx_ksteps(a->K) + c.unit - 1) / c.unit);
-        const double cost = c.us[b].fixed + c.us[b].first * units + (double)(rounds - 1) * (c.us[b].round + c.us[b].more * units);
-        if (c.unit > 1 && a->M > 65535 * (int64_t)c.rows) continue;      // the direct kernels' grid
-        if (i == MX_KINDS - 1 || cost < least) { best = i; least = cost; }
+    double least = mx_cost(a, best);
+    for (int i = MX_KINDS - 2; i >= 0; --i) {
+        if (MX_COST[i].unit > 1 && a->M > 65535 * (int64_t)MX_COST[i].rows) continue;      // the direct kernels' grid
+        const double cost = mx_cost(a, i);
+        if (cost < least) { best = i; least = cost; }
     }
     return (MxKind)best;
 }
 
-// The direct kernel quantises plain activations itself where a wave's share is one round of loads.  On the GPU alone the two
-// ways are near each other - 8 x 1280 x 1280 5.0 us fused, 5.8 as quantisation and product; 1 x 5120 x 5120 7.5 and 8.4; 1 x
-// 10240 x 5120 9.2 and 10.3; a second round of loads costs 2 us - and a launch less is 3 us less of the caller's time.
-static bool mx_fused(const sdmi_mx_gemm_args* a) {
-    return a->x && !a->algo && a->M <= MX_FUSED_PAIRS && a->M * ((mx_ksteps(a->K) + 7) / 8) <= MX_FUSED_PAIRS;
+// The direct kernel quantises plain activations itself where that is little work beside the product, since a launch less is 4 us
+// less of the caller's time (8 or 12 for an eager call) and about one on the GPU.  Each workgroup quantises its own rows, 16 (k-step,
+// row) pairs of a wave a trip, so the rule counts trips and rounds of workgroups on the 256 CUs.  GPU time alone, us, fused and
+// apart: one trip, 16 x 1280 x 1024 4.3 and 5.3, 1 x 10240 x 5120 7.6 and 9.1; three, 16 x 2560 x 2560 6.4 and 5.9; a second round
+// of workgroups, 16 x 20480 x 1024 7.6 and 7.9, but with more trips 8 x 20480 x 4096 15.1 and 12.9; 32 rows a workgroup where that
+// saves the second round, 231 x 1280 x 1024 6.6 and 6.2, 32 x 10240 x 1024 6.7 and 6.6.
+enum MxFused { MX_APART, MX_FUSED16x32, MX_FUSED16x64, MX_FUSED32x64 };
+static MxFused mx_fused(const sdmi_mx_gemm_args* a) {
+    if (!a->x || a->algo || a->M > 8192 || a->K % 8) return MX_APART;            // (eight values are a lane's load)
+    int64_t rows = 1;                                                            // of a workgroup, as the kernel counts them
+    while (rows < 16 && rows < a->M) rows *= 2;
+    const int64_t trips = (rows * ((mx_ksteps(a->K) + 7) / 8) + 15) / 16, r16 = (a->M + 15) / 16, c64 = (a->N + 63) / 64;
+    if (trips > 3) return MX_APART;
+    if (r16 * ((a->N + 31) / 32) <= 256) return MX_FUSED16x32;
+    if (r16 * c64 <= 256) return MX_FUSED16x64;
+    if (trips > 1) return MX_APART;
+    if ((r16 + 1) / 2 * c64 <= 256) return MX_FUSED32x64;
+    return r16 * c64 <= 512 ? MX_FUSED16x64 : MX_APART;
 }
 
 extern "C" int64_t sdmi_mx_gemm_workspace_bytes(const sdmi_mx_gemm_args* a) {
@@ -718,7 +756,7 @@ template <int FMT, int BM, int WGM, int WGN, int ST> static int tiled_launch(con
 }
 
 template <int FMT, int MT, int NF, int KW, int U, int SRC> static int direct_launch(const MxGemmDev& d, hipStream_t st) {
-    const int sums = KW * MT * NF * 1024, codes = SRC < 0 ? 0 : (int)(d.ksteps * d.M * (mx_row_bytes(128, FMT) + 4));
+    const int sums = KW * MT * NF * 1024, codes = SRC < 0 ? 0 : (int)(d.ksteps * (d.M < 16 * MT ? d.M : 16 * MT) * (mx_row_bytes(128, FMT) + 4));
     const int64_t nx = (d.N + 63) / 64 * (4 / NF), ny = (d.M + 16 * MT - 1) / (16 * MT);
     if (ny > 65535) return SDMI_ERR_BAD_ARG;
     sdmi_mx_direct_kernel<FMT, MT, NF, KW, U, SRC><<<dim3((unsigned)nx, (unsigned)ny), 64 * KW, sums > codes ? sums : codes, st>>>(d);
@@ -726,10 +764,17 @@ template <int FMT, int MT, int NF, int KW, int U, int SRC> static int direct_lau
     return SDMI_OK;
 }
 
-template <int FMT> static int mx_launch(const MxGemmDev& d, MxKind kind, int src, hipStream_t st) {
-    // quantising: 64 columns a workgroup where 32 would make more than one for each CU (1 x 10240 x 2560: 8.4 -> 7.1 us)
-    if (src >= 0 && d.N > 256 * 32) return src == 0 ? direct_launch<FMT, 1, 4, 8, 2, 0>(d, st) : src == 1 ? direct_launch<FMT, 1, 4, 8, 2, 1>(d, st) : direct_launch<FMT, 1, 4, 8, 2, 2>(d, st);
-    if (src >= 0) return src == 0 ? direct_launch<FMT, 1, 2, 8, 2, 0>(d, st) : src == 1 ? direct_launch<FMT, 1, 2, 8, 2, 1>(d, st) : direct_launch<FMT, 1, 2, 8, 2, 2>(d, st);
+template <int FMT, int MT, int NF> static int direct_fused(const MxGemmDev& d, int src, hipStream_t st) {
+    return src == 0 ? direct_launch<FMT, MT, NF, 8, 2, 0>(d, st) : src == 1 ? direct_launch<FMT, MT, NF, 8, 2, 1>(d, st) : direct_launch<FMT, MT, NF, 8, 2, 2>(d, st);
+}
+
+template <int FMT> static int mx_launch(const MxGemmDev& d, MxKind kind, MxFused fused, int src, hipStream_t st) {
+    switch (fused) {
+        case MX_FUSED16x32: return direct_fused<FMT, 1, 2>(d, src, st);
+        case MX_FUSED16x64: return direct_fused<FMT, 1, 4>(d, src, st);
+        case MX_FUSED32x64: return direct_fused<FMT, 2, 4>(d, src, st);
+        default: break;
+    }
     switch (kind) {
         case MX_D16x32: return direct_launch<FMT, 1, 2, 8, 2, -1>(d, st);
         case MX_D16x64: return direct_launch<FMT, 1, 4, 8, 2, -1>(d, st);
@@ -759,9 +804,9 @@ extern "C" int sdmi_mx_gemm(const sdmi_mx_gemm_args* a, void* stream) {
     if (need > 0 && (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace))) return SDMI_ERR_WORKSPACE;
     MxGemmDev d = {};
     d.xc = (const unsigned char*)a->x_codes; d.xs = (const unsigned char*)a->x_scales;
-    int src = -1;
-    if (mx_fused(a)) {
-        src = mx_src_type(a->x_dtype);
+    const MxFused fused = mx_fused(a);
+    const int src = fused ? mx_src_type(a->x_dtype) : -1;
+    if (fused) {
         d.x = a->x; d.ldx = a->ldx;
     } else if (a->x) {
         unsigned char* const ws = (unsigned char*)a->workspace;
@@ -774,5 +819,5 @@ extern "C" int sdmi_mx_gemm(const sdmi_mx_gemm_args* a, void* stream) {
     d.bias = a->bias; d.res = a->res; d.out = a->out;
     d.M = a->M; d.N = a->N; d.K = a->K; d.ksteps = mx_ksteps(a->K); d.ld_res = a->ld_res; d.ld_out = a->ld_out;
     d.type = type;
-    return a->fmt == SDMI_MX_FP8 ? mx_launch<SDMI_MX_FP8>(d, mx_kind(a), src, (hipStream_t)stream) : mx_launch<SDMI_MX_FP4>(d, mx_kind(a), src, (hipStream_t)stream);
+    return a->fmt == SDMI_MX_FP8 ? mx_launch<SDMI_MX_FP8>(d, mx_kind(a), fused, src, (hipStream_t)stream) : mx_launch<SDMI_MX_FP4>(d, mx_kind(a), fused, src, (hipStream_t)stream);
 }

@@ -343,6 +343,27 @@ def test_every_kernel_adds_and_rounds_once(dev, monkeypatch, algo, dtype):
             assert bool((wide[:, :pad] == 7.0).all()) and bool((wide[:, pad + n:] == 7.0).all()), (m, n, pad)
 
 
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_quantisation_inside_the_product(dev, fmt, dtype):
+    """Plain activations that the product quantises itself: the direct kernels' products of what mx_quantize gives, bit for bit
+    (their order of sums is one and the same).  Row counts around the powers of two and the tiles, K that ends in a k-step, in a
+    block and past the waves' first, second and third k-steps, and rows of any stride whose neighbours are NaN."""
+    o = ops()
+    for i, (m, n, k) in enumerate([(1, 40, 8), (1, 17000, 136), (3, 130, 1000), (5, 64, 5000), (8, 10300, 1056), (16, 100, 3064), (17, 300, 1032), (33, 1000, 1024),
+                                   (100, 4000, 40), (230, 1290, 1016), (257, 1100, 512), (31, 9000, 904), (40, 10000, 968), (300, 70, 2048), (900, 64, 256)]):
+        x = data(m, k, i, dtype, loud=i % 2 == 0)
+        pw = o.pack_linear_mx(torch.randn(n, k, generator=torch.Generator().manual_seed(i)).to(dev) * k ** -0.5)
+        q = o.mx_quantize(x.to(dev), fmt)
+        o.FORCE_MX_ALGO = 1
+        try:
+            want = o.linear_mx(q, pw, out_dtype=torch.float32)
+        finally:
+            o.FORCE_MX_ALGO = 0
+        for pad in (0, 3, 8):
+            assert torch.equal(o.linear_mx(strided(x, dev, pad), pw, fmt=fmt, out_dtype=torch.float32), want), (m, n, k, pad)
+
+
 @pytest.mark.parametrize("m", [1, 20, 150])
 @pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
 def test_linear_mx_picks_single_elements(dev, fmt, m):
