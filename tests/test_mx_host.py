@@ -101,11 +101,13 @@ def test_product_refusals(lib):
     assert lib.sdmi_mx_gemm(None, None) == BAD
     for bad in (dict(w_codes=P + 8), dict(w_scales=P + 2), dict(x=None, x_codes=P + 8, x_scales=P)):
         assert g(M=4, **bad) == ALIGN, bad
-    need = lib.sdmi_mx_gemm_workspace_bytes(C.byref(_gemm(M=300, K=1000, ldx=1000)))
+    # (a product that quantises by itself - K in whole eights, few tokens - has no use for a workspace)
+    assert lib.sdmi_mx_gemm_workspace_bytes(C.byref(_gemm(M=300, K=1000, ldx=1000))) == 0
+    need = lib.sdmi_mx_gemm_workspace_bytes(C.byref(_gemm(M=300, K=1001, ldx=1001)))
     assert need > 0
-    assert g(M=300, K=1000, ldx=1000) == WORKSPACE
-    assert g(M=300, K=1000, ldx=1000, workspace=P, workspace_bytes=need - 1) == WORKSPACE
-    assert g(M=300, K=1000, ldx=1000, workspace=P + 4, workspace_bytes=need) == WORKSPACE
+    assert g(M=300, K=1001, ldx=1001) == WORKSPACE
+    assert g(M=300, K=1001, ldx=1001, workspace=P, workspace_bytes=need - 1) == WORKSPACE
+    assert g(M=300, K=1001, ldx=1001, workspace=P + 4, workspace_bytes=need) == WORKSPACE
     assert lib.sdmi_mx_gemm_workspace_bytes(C.byref(_gemm(M=4, K=0))) == -1
 
 
