@@ -8,9 +8,7 @@
 // Packed weights: per group of 64 output columns and k-step of 128, four fragments of 64 lanes x 16 bytes, then (in a second
 // buffer) 64 lanes x 4 scale bytes, one for each fragment (the instruction selects the byte).  Fragment f, row 4 g + r holds
 // column 32 (f / 2) + 8 g + 4 (f % 2) + r of its group: the accumulator quads of fragments 0 and 1 (2 and 3) are then 8
-// CONSECUTIVE columns of a lane, 16 bytes of a 16-bit output, and the four lanes of a token store 64 bytes in one piece
-// (fp32 output of 4096 x 10240 x 1280: 86 us, and
-// 98 with 16 consecutive columns a lane, whose 16-byte pieces lie 64 apart).
+// CONSECUTIVE columns of a lane, 16 bytes of a 16-bit output, and the four lanes of a token have 64 bytes in one piece.
 #include "sdmi_mx.h"
 #include <type_traits>
 

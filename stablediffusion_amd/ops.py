@@ -967,12 +967,12 @@ def rmsnorm(x, gamma, eps=1e-6, res=None, fmt=None, out_dtype=None):
     if res is not None:
         if res.dtype != x.dtype or res.shape != x.shape:
             raise hip.SdmiError(f"rmsnorm: res is {res.dtype} {tuple(res.shape)}, x {x.dtype} {tuple(x.shape)}")
-        ld_res = _mx_rows(res, "res")[2]
+        ld_res = ld if res.stride() == x.stride() else _mx_rows(res, "res")[2]
         s = torch.empty_like(x, memory_format=torch.contiguous_format)
     if gamma.device != x.device or (res is not None and res.device != x.device):
         raise hip.SdmiError(f"rmsnorm: gamma and res have to be on x's device, {x.device}")
     if fmt is None:
-        y = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
+        y = torch.empty_like(x, dtype=out_dtype, memory_format=torch.contiguous_format)      # (0.8 us less than torch.empty)
         out, scales, code, odt = y.data_ptr(), None, hip.MX_NONE, _mx_dt(y.dtype, "rmsnorm out_dtype")
     else:
         if out_dtype is not None:
