@@ -477,7 +477,7 @@ typedef struct sdmi_mx_gemm_args {
     int32_t x_dtype, out_dtype;
     int32_t fmt;             /* of the activations */
     int32_t algo;            /* 0: the library picks the kernel; 1 ... SDMI_MX_ALGOS pins one (tests, measurements): the direct
-                                kernels of 16 x 32, 16 x 64, 48 x 32, 64 x 32 outputs a workgroup, the tiled ones of 64 x 128,
+                                kernels of 16 x 32, 16 x 64, 32 x 64, 48 x 64 outputs a workgroup, the tiled ones of 64 x 128,
                                 128 x 128, 128 x 256, 256 x 256 */
 } sdmi_mx_gemm_args;
 int64_t sdmi_mx_gemm_workspace_bytes(const sdmi_mx_gemm_args* args);   /* -1: sizes that sdmi_mx_gemm refuses */

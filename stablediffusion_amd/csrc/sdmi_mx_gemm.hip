@@ -291,14 +291,23 @@ __global__ __launch_bounds__(64 * KW) void sdmi_mx_direct_kernel(MxGemmDev p) {
     };
     if (mine > 0) load(0, 0);
     if (mine > U) load(1, U);
-    // one quad of the output for each lane of the first MT NF waves; its bias and residual travel behind the first weights
-    static_assert(MT * NF <= KW, "a wave stores one fragment");
-    const int of = f0 + wave % NF;
-    const int64_t om = m0 + wave / NF * 16 + row, on = grp * 64 + 32 * (of >> 1) + 8 * q + 4 * (of & 1);
-    const bool stores = wave < MT * NF && om < p.M && on < p.N;
-    uint4 bias = {0u, 0u, 0u, 0u}, res = bias;
-    if (stores && p.bias) bias = mx_quad_load(p.bias, on, 2, p.N - on);
-    if (stores && p.res) res = mx_quad_load(p.res, om * p.ld_res + on, p.type, p.N - on);
+    // the wave stores fragments wave, wave + KW ... of the output; their bias and residual travel behind the first weights
+    constexpr int OWN = (MT * NF + KW - 1) / KW;
+    auto place = [&](int i, int64_t& m, int64_t& n) {
+        const int t = wave + i * KW, f = f0 + t % NF;
+        m = m0 + t / NF * 16 + row;
+        n = grp * 64 + 32 * (f >> 1) + 8 * q + 4 * (f & 1);
+        return t < MT * NF && m < p.M && n < p.N;
+    };
+    uint4 bias[OWN], res[OWN];
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+        int64_t m, n;
+        const bool stores = place(i, m, n);
+        bias[i] = res[i] = (uint4){0u, 0u, 0u, 0u};
+        if (stores && p.bias) bias[i] = mx_quad_load(p.bias, n, 2, p.N - n);
+        if (stores && p.res) res[i] = mx_quad_load(p.res, m * p.ld_res + n, p.type, p.N - n);
+    }
     unsigned char* const own = smem;                       // SRC >= 0: [nk][rows][RB] codes, then [nk][rows][4] scales
     const int rows = (int)min(p.M - m0, (int64_t)(16 * MT));
     unsigned char* const own_s = smem + nk * rows * RB;
@@ -371,13 +380,17 @@ __global__ __launch_bounds__(64 * KW) void sdmi_mx_direct_kernel(MxGemmDev p) {
 #pragma unroll
         for (int f = 0; f < NF; ++f) part[((wave * MT + mi) * NF + f) * 64 + lane] = acc[mi][f];
     __syncthreads();
-    if (stores) {
-        f32x4 v = part[wave * 64 + lane];
 #pragma unroll
-        for (int k = 1; k < KW; ++k) v += part[(k * MT * NF + wave) * 64 + lane];
-        if (p.bias) v += mx_quad_values(bias, 2);
-        if (p.res) v += mx_quad_values(res, p.type);
-        mx_quad_store(p, om, on, v);
+    for (int i = 0; i < OWN; ++i) {
+        int64_t m, n;
+        if (!place(i, m, n)) continue;
+        const int t = wave + i * KW;
+        f32x4 v = part[t * 64 + lane];
+#pragma unroll
+        for (int k = 1; k < KW; ++k) v += part[(k * MT * NF + t) * 64 + lane];
+        if (p.bias) v += mx_quad_values(bias[i], 2);
+        if (p.res) v += mx_quad_values(res[i], p.type);
+        mx_quad_store(p, m, n, v);
     }
 }
 
@@ -665,29 +678,33 @@ static bool mx_args_ok(const sdmi_mx_gemm_args* a) {
 // Which kernel runs a product: the cheapest by a model of rounds.  A kernel's workgroups take `rows` x `cols` of the output; a
 // launch costs `fixed` us, a unit of K `first` for the first workgroup on each of the 256 CUs, and every further round of them
 // `round` and `more` a unit.  (Direct kernels: the unit is eight k-steps, one for each wave; tiled ones: one k-step.)  Least
-// squares over a sweep of 1 ... 8192 rows and fourteen (N, K) from 320 x 320 to 10240 x 5120 and 2560 x 10240, of each kernel
-// where it takes at most twice as long as the fastest; the kernel picked is within 1 % of the fastest one on average and 24 % at
-// worst (1 x 1280 x 1280, a microsecond).  Examples, us, 8-bit activations (direct kernels by their outputs a workgroup, D, tiled
-// ones T):
-//     48 x  5120 x 5120: D 16 x 64  7.6, D 48 x 32  9.2, D 16 x 32  9.2, T 64 x 128 15.1
-//    256 x  1280 x 1280: D 48 x 32  5.0, T 64 x 128  6.6, T 128 x 128  8.5
-//    512 x  5120 x 1280: T 128 x 128  9.4, T 64 x 128  9.4, T 256 x 256 17.0, D 64 x 32 18.6
-//   1024 x  5120 x 5120: T 64 x 128 30.6, T 128 x 256 31.6, T 128 x 128 33.4, T 256 x 256 47.9
-//   4096 x  5120 x 5120: T 128 x 128 85.1, T 64 x 128 96.8, T 256 x 256 102.9 (320 tiles: two rounds)
-//   8192 x  5120 x 5120: T 256 x 256 171, T 128 x 256 177, T 128 x 128 190
+// squares over a sweep of 1 ... 8192 rows and fifteen (N, K) from 320 x 320 to 10240 x 5120 and 2560 x 10240, of each kernel
+// where it takes at most 1.3 times as long as the fastest; the kernel picked is within 0.6 % of the fastest one on average and
+// 26 % at worst (192 x 320 x 320, a microsecond).  Examples, us, 8-bit activations (direct kernels by their outputs a
+// workgroup, D, tiled ones T):
+//     32 x 10240 x 5120: D 32 x 64  9.4, D 48 x 64 10.4, D 16 x 64 12.4, D 16 x 32 12.7
+//     48 x  5120 x 5120: D 16 x 64  7.7, D 32 x 64  8.4, D 16 x 32  9.2, D 48 x 64 10.4
+//    128 x  5120 x 5120: D 48 x 64 10.8, D 32 x 64 14.1, T 64 x 128 15.4, T 128 x 128 21.0
+//    256 x  1280 x 1280: D 32 x 64  4.9, D 48 x 64  5.5, T 64 x 128  6.7, T 128 x 128  8.5
+//    512 x  5120 x 1280: T 128 x 128  9.4, T 64 x 128  9.5, D 48 x 64 15.8, T 256 x 256 16.9
+//   1024 x  5120 x 5120: T 64 x 128 30.7, T 128 x 256 30.9, T 128 x 128 32.5, T 256 x 256 47.7
+//   4096 x  5120 x 5120: T 128 x 128 84.9, T 64 x 128 96.9, T 256 x 256 102.4 (320 tiles: two rounds)
+//   8192 x  5120 x 5120: T 256 x 256 161, T 128 x 256 170, T 128 x 128 183
+// Activations are read again by every column group and weights by every row tile, from L2, which is what the direct kernels'
+// shapes trade (96 x 5120 x 5120: 48 x 32 and 64 x 32 15.2 and 15.3 us, 32 x 64 8.9).
 // Parts of K in several workgroups of a tiled kernel and a second launch that joins them were measured too (two and four parts)
 // and won by 6 % at most, at one size: the workgroups of a direct kernel split K among their waves already.
-enum MxKind { MX_D16x32, MX_D16x64, MX_D48x32, MX_D64x32, MX_T64x128, MX_T128x128, MX_T128x256, MX_T256x256, MX_KINDS };
+enum MxKind { MX_D16x32, MX_D16x64, MX_D32x64, MX_D48x64, MX_T64x128, MX_T128x128, MX_T128x256, MX_T256x256, MX_KINDS };
 struct MxCost { int rows, cols, unit; struct { double fixed, first, round, more; } us[2]; };      // [0]: 8-bit activations, [1]: 4-bit
 static const MxCost MX_COST[MX_KINDS] = {
-    {16, 32, 8, {{3.542, 0.412, 0.157, 0.480}, {3.537, 0.340, 0.214, 0.345}}},
-    {16, 64, 8, {{3.449, 0.624, 0.482, 0.716}, {3.514, 0.528, 0.492, 0.567}}},
-    {48, 32, 8, {{3.440, 0.820, 0.596, 1.134}, {3.554, 0.519, 0.537, 0.791}}},
-    {64, 32, 8, {{3.377, 1.059, 0.544, 1.449}, {3.506, 0.681, 0.736, 0.997}}},
-    {64, 128, 1, {{4.086, 0.278, 0.939, 0.200}, {4.048, 0.257, 0.929, 0.147}}},
-    {128, 128, 1, {{4.530, 0.426, 1.462, 0.360}, {4.415, 0.331, 1.710, 0.220}}},
-    {128, 256, 1, {{5.473, 0.610, 4.259, 0.748}, {5.428, 0.452, 4.360, 0.541}}},
-    {256, 256, 1, {{6.915, 1.100, 6.615, 1.250}, {6.885, 0.647, 6.995, 0.833}}},
+    {16, 32, 8, {{3.636, 0.403, 0.006, 0.500}, {3.538, 0.341, 0.109, 0.367}}},
+    {16, 64, 8, {{3.496, 0.618, 0.396, 0.727}, {3.550, 0.500, 0.308, 0.633}}},
+    {32, 64, 8, {{3.377, 0.876, 0.909, 1.010}, {3.525, 0.630, 0.659, 0.775}}},
+    {48, 64, 8, {{3.395, 1.180, 0.706, 1.436}, {3.654, 0.812, 1.138, 0.962}}},
+    {64, 128, 1, {{4.050, 0.286, 0.984, 0.193}, {4.015, 0.265, 0.975, 0.137}}},
+    {128, 128, 1, {{4.844, 0.423, 1.385, 0.351}, {4.606, 0.329, 1.706, 0.216}}},
+    {128, 256, 1, {{6.283, 0.625, 3.900, 0.717}, {6.293, 0.448, 3.865, 0.543}}},
+    {256, 256, 1, {{8.431, 1.113, 6.373, 1.182}, {8.274, 0.653, 6.362, 0.811}}},
 };
 static_assert(MX_KINDS == SDMI_MX_ALGOS, "sdmi_mx_gemm_args.algo");
 static int64_t mx_rounds(const sdmi_mx_gemm_args* a, int kind) {
@@ -757,6 +774,11 @@ template <int FMT, int MT, int NF, int KW, int U, int SRC> static int direct_lau
     const int sums = KW * MT * NF * 1024, codes = SRC < 0 ? 0 : (int)(d.ksteps * (d.M < 16 * MT ? d.M : 16 * MT) * (mx_row_bytes(128, FMT) + 4));
     const int64_t nx = (d.N + 63) / 64 * (4 / NF), ny = (d.M + 16 * MT - 1) / (16 * MT);
     if (ny > 65535) return SDMI_ERR_BAD_ARG;
+    if (KW * MT * NF * 1024 > 65536) {
+        static SdmiPerDeviceOnce once;
+        const int r = once.run([&] { return hipFuncSetAttribute(reinterpret_cast<const void*>(sdmi_mx_direct_kernel<FMT, MT, NF, KW, U, SRC>), hipFuncAttributeMaxDynamicSharedMemorySize, KW * MT * NF * 1024) == hipSuccess; });
+        if (r != SDMI_OK) return r;
+    }
     sdmi_mx_direct_kernel<FMT, MT, NF, KW, U, SRC><<<dim3((unsigned)nx, (unsigned)ny), 64 * KW, sums > codes ? sums : codes, st>>>(d);
     SDMI_CHECK_LAUNCH();
     return SDMI_OK;
@@ -776,8 +798,8 @@ template <int FMT> static int mx_launch(const MxGemmDev& d, MxKind kind, MxFused
     switch (kind) {
         case MX_D16x32: return direct_launch<FMT, 1, 2, 8, 2, -1>(d, st);
         case MX_D16x64: return direct_launch<FMT, 1, 4, 8, 2, -1>(d, st);
-        case MX_D48x32: return direct_launch<FMT, 3, 2, 8, 1, -1>(d, st);
-        case MX_D64x32: return direct_launch<FMT, 4, 2, 8, 1, -1>(d, st);
+        case MX_D32x64: return direct_launch<FMT, 2, 4, 8, 1, -1>(d, st);
+        case MX_D48x64: return direct_launch<FMT, 3, 4, 8, 1, -1>(d, st);
         // Rings no deeper than leaves room for three workgroups on a CU, whose starts and stores then run under each other's
         // products (4096 x 10240 x 1280, 64 x 128: 8 bits 76.8 -> 69.5 us, 4 bits 62.0 -> 53.5; 128 x 128, 4 bits 48.9 -> 44.8); with
         // 8-bit operands that is two stages of 128 x 128, which wait for their loads when they are alone on a CU
