@@ -123,8 +123,8 @@ __device__ __forceinline__ void mx_quad_store(const MxGemmDev& p, int64_t m, int
 // 16-bit types columns c and c + 32, of fp32 c and c + 4) go round the lanes until lane l holds piece l % 8 of a 128-byte line of
 // token l / 8, in the first of the two for tokens 0 ... 7 of the fragment and in the second for 8 ... 15; residuals take the same
 // way back.  (8192 x 10240 x 1280, 256 x 256 tiles, us: 4 bits 90 -> 86, with residual 121 -> 117; 4096 x 10240 x 1280 fp32
-// 86 -> 79.  Stores past the caches were faster by themselves, 72 for 86, but whatever reads the output next then fetches it from memory:
-// 8192 x 10240 x 5120 with the quantisation of its output 235 us, and 243 like that.)
+// 86 -> 79.  Stores past the caches gain nothing, and whatever reads the output next has to fetch it from memory: 8192 x 10240 x
+// 5120 with the quantisation of its output 241 us, and 232 like this.)
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 __attribute__((aligned(2))) mx_u32x4_a2;
 __device__ __forceinline__ void mx_swap_rows(u32x4& a, u32x4& b, bool upper) {       // rows 0 - 7's b for rows 8 - 15's a; its own inverse
@@ -443,11 +443,13 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void sdmi_mx_tiled_kernel(MxGemm
 
     // Workgroups go round the 8 XCDs; each XCD takes a run of consecutive tiles, and a run walks BAND token tiles before the next
     // column tile, so that the tiles an XCD works on together - 32 of 256 x 256, 64 of the smaller ones - are a compact patch
-    // and share their operands in its L2 (8192 x 8192 x 8192 in 8 bits: BAND 2 362 us, 4 354, 8 363, 16 369, 32 405).
+    // and share their operands in its L2.  Heights that are no power of two: with 4 or 8 the runs of all XCDs start in the same
+    // column tile of their bands and write lines a power of two apart at a time (8192 x 10240 x 1280, 4 bits: 256 x 256 tiles
+    // 86 us with 4, 76 with 5, 128 x 128 ones 96 with 8, 79 with 7; 4096 x 5120 x 5120 the same with either).
     const unsigned tm = (unsigned)((p.M + BM - 1) / BM), tn = (unsigned)((p.N + T::BN - 1) / T::BN), total = tm * tn;
     const unsigned xcd = blockIdx.x & 7, each = total >> 3, more = total & 7;
     const unsigned id = (xcd < more ? xcd * (each + 1) : more + xcd * each) + (blockIdx.x >> 3);
-    constexpr unsigned BAND = BM == 256 ? 4 : 8;
+    constexpr unsigned BAND = BM == 256 ? 5 : 7;
     const unsigned band = id / (BAND * tn), height = min(BAND, tm - band * BAND), in_band = id - band * BAND * tn;
     const int64_t m0 = (int64_t)(band * BAND + in_band % height) * BM;
     const int64_t g0 = (int64_t)(in_band / height) * WGN, groups = (p.N + 63) >> 6;
@@ -679,8 +681,8 @@ static bool mx_args_ok(const sdmi_mx_gemm_args* a) {
 // launch costs `fixed` us, a unit of K `first` for the first workgroup on each of the 256 CUs, and every further round of them
 // `round` and `more` a unit.  (Direct kernels: the unit is eight k-steps, one for each wave; tiled ones: one k-step.)  Least
 // squares over a sweep of 1 ... 8192 rows and fifteen (N, K) from 320 x 320 to 10240 x 5120 and 2560 x 10240, of each kernel
-// where it takes at most 1.3 times as long as the fastest; the kernel picked is within 0.6 % of the fastest one on average and
-// 26 % at worst (192 x 320 x 320, a microsecond).  Examples, us, 8-bit activations (direct kernels by their outputs a
+// where it takes at most 1.3 times as long as the fastest; the kernel picked is within 0.4 % of the fastest one on average and
+// 14 % at worst (1 x 640 x 640, 0.6 us).  Examples, us, 8-bit activations (direct kernels by their outputs a
 // workgroup, D, tiled ones T):
 //     32 x 10240 x 5120: D 32 x 64  9.4, D 48 x 64 10.4, D 16 x 64 12.4, D 16 x 32 12.7
 //     48 x  5120 x 5120: D 16 x 64  7.7, D 32 x 64  8.4, D 16 x 32  9.2, D 48 x 64 10.4
@@ -689,7 +691,7 @@ static bool mx_args_ok(const sdmi_mx_gemm_args* a) {
 //    512 x  5120 x 1280: T 128 x 128  9.4, T 64 x 128  9.5, D 48 x 64 15.8, T 256 x 256 16.9
 //   1024 x  5120 x 5120: T 64 x 128 30.7, T 128 x 256 30.9, T 128 x 128 32.5, T 256 x 256 47.7
 //   4096 x  5120 x 5120: T 128 x 128 84.9, T 64 x 128 96.9, T 256 x 256 102.4 (320 tiles: two rounds)
-//   8192 x  5120 x 5120: T 256 x 256 161, T 128 x 256 170, T 128 x 128 183
+//   8192 x  5120 x 5120: T 256 x 256 164, T 128 x 256 171, T 128 x 128 174
 // Activations are read again by every column group and weights by every row tile, from L2, which is what the direct kernels'
 // shapes trade (96 x 5120 x 5120: 48 x 32 and 64 x 32 15.2 and 15.3 us, 32 x 64 8.9).
 // Parts of K in several workgroups of a tiled kernel and a second launch that joins them were measured too (two and four parts)
