@@ -245,7 +245,6 @@ template <> struct MxRaw8<2> {
 // registers, U k-steps ahead of the ones they multiply, and join their sums through LDS in a fixed order.
 // SRC >= 0: x is a plain matrix of that type (mx_src_type), of which every workgroup quantises its rows for itself (mx_fused),
 // into LDS while its first weights are on their way: one launch instead of two.
-
 template <int FMT, int MT, int NF, int KW, int U, int SRC>
 __global__ __launch_bounds__(64 * KW) void sdmi_mx_direct_kernel(MxGemmDev p) {
     extern __shared__ unsigned char smem[];
@@ -546,6 +545,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void sdmi_mx_tiled_kernel(MxGemm
     // publishes Y of this k-step and X of the next, the slots also issue the next fill and read the weights and first
     // activations of k-step s + 1.  So the matrix pipe waits neither for a burst of loads nor for LDS behind the barrier.
     constexpr int AHEAD = 1, TURN = T::HALF - AHEAD, SLOTS = T::MF - TURN;
+    static_assert(TURN >= 0, "the slot of the wait and the barrier");
     struct Act { uint4 a, b; int s; };
     struct Step { uint4 w[4]; int ws; Act x[AHEAD]; };
     auto read_act = [&](const unsigned char* st, int mi) {
