@@ -680,9 +680,9 @@ static bool mx_args_ok(const sdmi_mx_gemm_args* a) {
 // Which kernel runs a product: the cheapest by a model of rounds.  A kernel's workgroups take `rows` x `cols` of the output; a
 // launch costs `fixed` us, a unit of K `first` for the first workgroup on each of the 256 CUs, and every further round of them
 // `round` and `more` a unit.  (Direct kernels: the unit is eight k-steps, one for each wave; tiled ones: one k-step.)  Least
-// squares over a sweep of 1 ... 8192 rows and fifteen (N, K) from 320 x 320 to 10240 x 5120 and 2560 x 10240, of each kernel
-// where it takes at most 1.3 times as long as the fastest; the kernel picked is within 0.4 % of the fastest one on average and
-// 14 % at worst (1 x 640 x 640, 0.6 us).  Examples, us, 8-bit activations (direct kernels by their outputs a
+// squares over a sweep of 1 ... 8192 rows and twenty (N, K) from 320 x 320 to 20480 x 2560 and 5120 x 10240, of each kernel
+// where it takes at most 1.3 times as long as the fastest; the kernel picked is within 0.5 % of the fastest one on average and
+// 13 % at worst (1 x 640 x 640, 0.6 us).  Examples, us, 8-bit activations (direct kernels by their outputs a
 // workgroup, D, tiled ones T):
 //     32 x 10240 x 5120: D 32 x 64  9.4, D 48 x 64 10.4, D 16 x 64 12.4, D 16 x 32 12.7
 //     48 x  5120 x 5120: D 16 x 64  7.7, D 32 x 64  8.4, D 16 x 32  9.2, D 48 x 64 10.4
@@ -699,14 +699,14 @@ static bool mx_args_ok(const sdmi_mx_gemm_args* a) {
 enum MxKind { MX_D16x32, MX_D16x64, MX_D32x64, MX_D48x64, MX_T64x128, MX_T128x128, MX_T128x256, MX_T256x256, MX_KINDS };
 struct MxCost { int rows, cols, unit; struct { double fixed, first, round, more; } us[2]; };      // [0]: 8-bit activations, [1]: 4-bit
 static const MxCost MX_COST[MX_KINDS] = {
-    {16, 32, 8, {{3.636, 0.403, 0.006, 0.500}, {3.538, 0.341, 0.109, 0.367}}},
-    {16, 64, 8, {{3.496, 0.618, 0.396, 0.727}, {3.550, 0.500, 0.308, 0.633}}},
-    {32, 64, 8, {{3.377, 0.876, 0.909, 1.010}, {3.525, 0.630, 0.659, 0.775}}},
-    {48, 64, 8, {{3.395, 1.180, 0.706, 1.436}, {3.654, 0.812, 1.138, 0.962}}},
-    {64, 128, 1, {{4.050, 0.286, 0.984, 0.193}, {4.015, 0.265, 0.975, 0.137}}},
-    {128, 128, 1, {{4.844, 0.423, 1.385, 0.351}, {4.606, 0.329, 1.706, 0.216}}},
-    {128, 256, 1, {{6.283, 0.625, 3.900, 0.717}, {6.293, 0.448, 3.865, 0.543}}},
-    {256, 256, 1, {{8.431, 1.113, 6.373, 1.182}, {8.274, 0.653, 6.362, 0.811}}},
+    {16, 32, 8, {{3.533, 0.425, 0.143, 0.475}, {3.547, 0.335, 0.280, 0.333}}},
+    {16, 64, 8, {{3.471, 0.615, 0.875, 0.599}, {3.600, 0.478, 0.631, 0.536}}},
+    {32, 64, 8, {{3.419, 0.865, 1.180, 0.968}, {3.572, 0.613, 0.824, 0.766}}},
+    {48, 64, 8, {{3.466, 1.178, 1.621, 1.235}, {3.741, 0.776, 1.520, 0.929}}},
+    {64, 128, 1, {{4.051, 0.287, 0.930, 0.194}, {4.027, 0.266, 0.928, 0.139}}},
+    {128, 128, 1, {{4.829, 0.430, 1.295, 0.352}, {4.602, 0.333, 1.540, 0.219}}},
+    {128, 256, 1, {{6.310, 0.625, 3.707, 0.733}, {6.323, 0.446, 3.612, 0.546}}},
+    {256, 256, 1, {{8.487, 1.145, 5.791, 1.232}, {8.405, 0.649, 6.026, 0.828}}},
 };
 static_assert(MX_KINDS == SDMI_MX_ALGOS, "sdmi_mx_gemm_args.algo");
 static int64_t mx_rounds(const sdmi_mx_gemm_args* a, int kind) {
