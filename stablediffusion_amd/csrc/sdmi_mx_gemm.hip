@@ -681,7 +681,7 @@ static bool mx_args_ok(const sdmi_mx_gemm_args* a) {
 // launch costs `fixed` us, a unit of K `first` for the first workgroup on each of the 256 CUs, and every further round of them
 // `round` and `more` a unit.  (Direct kernels: the unit is eight k-steps, one for each wave; tiled ones: one k-step.)  Least
 // squares over a sweep of 1 ... 8192 rows and twenty (N, K) from 320 x 320 to 20480 x 2560 and 5120 x 10240, of each kernel
-// where it takes at most 1.3 times as long as the fastest; the kernel picked is within 0.5 % of the fastest one on average and
+// where it takes at most 1.2 or 1.3 times as long as the fastest; the kernel picked is within 0.5 % of the fastest one on average and
 // 13 % at worst (1 x 640 x 640, 0.6 us).  Examples, us, 8-bit activations (direct kernels by their outputs a
 // workgroup, D, tiled ones T):
 //     32 x 10240 x 5120: D 32 x 64  9.4, D 48 x 64 10.4, D 16 x 64 12.4, D 16 x 32 12.7
@@ -703,10 +703,10 @@ static const MxCost MX_COST[MX_KINDS] = {
     {16, 64, 8, {{3.471, 0.615, 0.875, 0.599}, {3.600, 0.478, 0.631, 0.536}}},
     {32, 64, 8, {{3.419, 0.865, 1.180, 0.968}, {3.572, 0.613, 0.824, 0.766}}},
     {48, 64, 8, {{3.466, 1.178, 1.621, 1.235}, {3.741, 0.776, 1.520, 0.929}}},
-    {64, 128, 1, {{4.051, 0.287, 0.930, 0.194}, {4.027, 0.266, 0.928, 0.139}}},
-    {128, 128, 1, {{4.829, 0.430, 1.295, 0.352}, {4.602, 0.333, 1.540, 0.219}}},
-    {128, 256, 1, {{6.310, 0.625, 3.707, 0.733}, {6.323, 0.446, 3.612, 0.546}}},
-    {256, 256, 1, {{8.487, 1.145, 5.791, 1.232}, {8.405, 0.649, 6.026, 0.828}}},
+    {64, 128, 1, {{4.050, 0.286, 0.984, 0.193}, {4.069, 0.268, 1.036, 0.127}}},
+    {128, 128, 1, {{4.844, 0.423, 1.385, 0.351}, {4.808, 0.323, 1.480, 0.222}}},
+    {128, 256, 1, {{6.283, 0.625, 3.900, 0.717}, {6.287, 0.484, 3.799, 0.524}}},
+    {256, 256, 1, {{8.431, 1.113, 6.373, 1.182}, {8.944, 0.678, 6.108, 0.793}}},
 };
 static_assert(MX_KINDS == SDMI_MX_ALGOS, "sdmi_mx_gemm_args.algo");
 static int64_t mx_rounds(const sdmi_mx_gemm_args* a, int kind) {
