@@ -435,6 +435,7 @@ int sdmi_image_to_u8(const float* x, uint8_t* out, int32_t nb, int32_t C, int64_
  *       [rows, C] of out_dtype; else out holds codes, and scales the scales.
  *   sdmi_gated:         y = a * act(b), x = [a | b] with halves of `inner` columns (the order of the GEGLU projection,
  *       ldm/modules/attention.py:89); act 0 GELU (erf), 1 SiLU; fmt, out, scales as above.
+ *       Gates act(b) below the normal numbers of fp32 (2^-126) may be taken as 0.
  * ---------------------------------------------------------------------------------------- */
 #define SDMI_MX_NONE 0
 #define SDMI_MX_FP8 1

@@ -50,7 +50,7 @@ __global__ __launch_bounds__(256) void sdmi_mx_elem_kernel(MxElemArgs p) {
             for (int j = 0; j < 8; ++j) f[s][j] *= mx_gelu(g[s][j]);
         } else if constexpr (OP == 2) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[s][j] *= silu_f(g[s][j]);
+            for (int j = 0; j < 8; ++j) f[s][j] *= mx_silu<FMT < 0 && TO == 2>(g[s][j]);
         }
         if constexpr (FMT < 0) {
             if (row < p.rows && n > 0)
