@@ -129,12 +129,24 @@ template <int FMT> __device__ __forceinline__ unsigned mx_quantise8(const float*
     return dw;
 }
 
+// The gates.  Both are taken in hardware approximations of exp2 and 1 / x (one step of fp32 each), as 16-bit and block-scaled
+// results show nothing of their errors (half a step is 2^-12 of a value at least); F32, the form for fp32 results, takes out the one error
+// that grows with |x|, the rounding of the exponential's argument.
+
+// 2^-(c m) for m in [0, 200]: c m as a rounded product and its remainder, c in two parts; exact but for exp2's own step.
+__device__ __forceinline__ float mx_exp2_neg(float m, float c, float c_low) {
+    const float t = m * c, low = fmaf(m, c_low, fmaf(m, c, -t));
+    const float e = __builtin_amdgcn_exp2f(-t);
+    return fmaf(e, -0.69314718055994531f * low, e);
+}
+constexpr float MX_HALF_LOG2E = 0.72134752044448170f, MX_HALF_LOG2E_LOW = (float)(0.72134752044448170368 - (double)MX_HALF_LOG2E);
+
 // GELU by the error function, x Phi(x) = max(x, 0) - |x| Phi(-|x|), for any magnitude: Phi(-|x|) = erfc(z) / 2 with
 // z = |x| / sqrt 2, and erfc(z) = exp(-z^2) t P(t), t = 1 / (1 + 0.425 z), P a degree-7 polynomial fitted to exp(z^2) erfc(z)
 // on [0, 10] (relative error 1.45e-7; its halves stand below).  Written from the small side, so that the tail of negative x
 // keeps its relative precision, and in 15 plain and two transcendental instructions; 1.5 x 2^-24 off on average over standard
-// normal x (degree 6: 4.8, degree 8: 1.4).
-__device__ __forceinline__ float mx_gelu(float x) {
+// normal x (degree 6: 4.8, degree 8: 1.4), x^2 2^-24 further out.
+template <bool F32> __device__ __forceinline__ float mx_gelu(float x) {
     const float t = __builtin_amdgcn_rcpf(fmaf(0.425f * 0.70710678118654752f, fabsf(x), 1.0f));
     float p = fmaf(0.5f * 7.147743966e-02f, t, -0.5f * 3.131541818e-01f);
     p = fmaf(p, t, 0.5f * 4.076140037e-01f);
@@ -143,21 +155,27 @@ __device__ __forceinline__ float mx_gelu(float x) {
     p = fmaf(p, t, 0.5f * 2.007062229e-01f);
     p = fmaf(p, t, 0.5f * 2.418405982e-01f);
     p = fmaf(p, t, 0.5f * 2.396786286e-01f);
-    const float half = p * t * __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f);      // Phi(-|x|); exp(-z^2) = 2^(-x^2 / (2 ln 2))
-    return fmaf(-fminf(fabsf(x), 3e38f), half, fmaxf(x, 0.0f));                           // (infinity times 0 would be NaN)
+    if constexpr (F32) {
+        // exp(-z^2) = 2^-(c x^2) with x^2 as a rounded square and its remainder (nothing is left of it from 30 on)
+        const float m = fminf(fabsf(x), 30.0f), s = m * m, low = fmaf(fmaf(m, m, -s), -0.5f, 1.0f);
+        return fmaf(-(fminf(fabsf(x), 3e38f) * p * t), mx_exp2_neg(s, MX_HALF_LOG2E, MX_HALF_LOG2E_LOW) * low, fmaxf(x, 0.0f));
+    } else {
+        const float half = p * t * __builtin_amdgcn_exp2f(x * x * -MX_HALF_LOG2E);         // Phi(-|x|)
+        return fmaf(-fminf(fabsf(x), 3e38f), half, fmaxf(x, 0.0f));                       // (infinity times 0 would be NaN)
+    }
 }
 
 // SiLU, x / (1 + exp(-x)).  The result is a normal fp32 number down to x = -91.6, exp(-x) only up to 88.7 and its reciprocal to
-// 87.3, so both are taken 2^-8 smaller.  The last scaling rounds the reciprocal to 17 bits out there: F32, the form for fp32
-// results, writes it from exp(-|x|) = h^2 instead, whose root goes into the product twice (16384 x 5120 bf16, 4-bit result:
+// 87.3, so both are taken 2^-8 smaller.  The last scaling rounds the reciprocal to 17 bits out there: the form for fp32
+// results is written from exp(-|x|) = h^2 instead, whose root goes into the product twice (16384 x 5120 bf16, 4-bit result:
 // 88 us, and 91 in that form).
 template <bool F32> __device__ __forceinline__ float mx_silu(float x) {
     if constexpr (F32) {
-        const float h = __builtin_amdgcn_exp2f(fabsf(x) * -0.72134752044448170f);        // exp(-|x| / 2) = 2^(-|x| / (2 ln 2))
+        const float h = mx_exp2_neg(fminf(fabsf(x), 200.0f), MX_HALF_LOG2E, MX_HALF_LOG2E_LOW);       // exp(-|x| / 2)
         const float w = x < 0.0f ? h : 1.0f;
         return x * w * w * __builtin_amdgcn_rcpf(fmaf(h, h, 1.0f));
     } else {
-        const float e = __builtin_amdgcn_exp2f(fmaf(x, -1.44269504088896341f, -8.0f));
+        const float e = __builtin_amdgcn_exp2f(fmaf(x, -2.0f * MX_HALF_LOG2E, -8.0f));
         return x * (__builtin_amdgcn_rcpf(e + 0x1p-8f) * 0x1p-8f);
     }
 }

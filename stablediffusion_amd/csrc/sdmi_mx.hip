@@ -47,7 +47,7 @@ __global__ __launch_bounds__(256) void sdmi_mx_elem_kernel(MxElemArgs p) {
         const int n = (int)max((int64_t)0, min((int64_t)8, p.K - k0));
         if constexpr (OP == 1) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[s][j] *= mx_gelu(g[s][j]);
+            for (int j = 0; j < 8; ++j) f[s][j] *= mx_gelu<FMT < 0 && TO == 2>(g[s][j]);
         } else if constexpr (OP == 2) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[s][j] *= mx_silu<FMT < 0 && TO == 2>(g[s][j]);

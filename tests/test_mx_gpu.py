@@ -585,3 +585,24 @@ def test_silu_where_its_exponential_leaves_fp32(dev, dtype, fmt):
     else:
         y = ops().gated(torch.cat([a, b]).view(1, -1).to(dev), act="silu", fmt=fmt)
         assert O.held_within(ops().mx_dequantize(y).double().cpu(), want.view(1, -1), GATE_REL, fmt)
+
+
+# ----------------------------------------------------------------------------- what fp32 results hold
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+def test_gate_in_fp32(dev, act, dtype):
+    """fp32 results, whose errors do not grow with |x|.  In units of 2^-24 of the gate's value, at worst.  SiLU: exp2's one step
+    2, its exponent's remainder 1 and the product with it 1, all twice for the square, 1 + h^2 1, its reciprocal 2, three
+    products 3, the gate's product 1: 15 < 16.  GELU: the fit 2.4; t = 1 / (1 + 0.3 |x|) 4 (constant, sum, a reciprocal's one
+    step), and exp(z^2) erfc(z) moves by 2.65 times that at z = 0, less further out, 10.6; the polynomial's seven sums, whose terms
+    are up to 1.8 times the value, 7; exp2 2, the square's and the exponent's remainders 2, five products 5, the gate's 1: 30 < 32."""
+    rel = (32 if act == "gelu" else 16) * 2.0 ** -24
+    lo = -13.0 if act == "gelu" else -91.5                     # (Phi leaves the normal numbers at -13.1)
+    for b in (torch.linspace(lo, 13.0, 6000), torch.linspace(-2.0, 2.0, 6000), torch.randn(6000, generator=torch.Generator().manual_seed(1))):
+        b = b.to(TYPES[dtype])
+        b = b[b >= lo]
+        for a in (1.0, -3.0):
+            y = ops().gated(torch.stack([torch.full_like(b, a), b], 1).to(dev), act=act, out_dtype=torch.float32).view(-1)
+            within(y, a * O.gate(b.double(), act), rel, torch.float32)
