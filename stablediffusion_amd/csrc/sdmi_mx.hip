@@ -179,10 +179,13 @@ __global__ __launch_bounds__(256) void sdmi_rmsnorm_kernel(MxNormArgs p) {
 #pragma unroll
         for (int w = 0; w < TPR / 64; ++w) ss += part[r][w];
     }
-    // 1 / sqrt(v), one Newton step from the approximation, as the sum of two fp32 numbers
+    // 1 / sqrt(v), one Newton step from the approximation, as the sum of two fp32 numbers.  Of rows of subnormals it lies past
+    // fp32's largest number, of rows near that one among the subnormals: there `up` brings it back, and the values with it.
     const double v = ss * p.inv_c + (double)p.eps;
     double r1 = __builtin_amdgcn_rsq(v);
     if (v > 0.0 && v < 1e300) r1 *= fma(-0.5 * v * r1, r1, 1.5);
+    const float up = r1 > 0x1p96 ? 0x1p64f : r1 < 0x1p-96 ? 0x1p-64f : 1.0f;
+    r1 *= r1 > 0x1p96 ? 0x1p-64 : r1 < 0x1p-96 ? 0x1p64 : 1.0;
     const float r0 = (float)r1, lo = r0 < 3e38f ? (float)(r1 - (double)r0) : 0.0f;
     const int64_t nsteps = mx_ksteps(p.C);
 #pragma unroll
@@ -194,7 +197,10 @@ __global__ __launch_bounds__(256) void sdmi_rmsnorm_kernel(MxNormArgs p) {
         float gm[8];
         mx_load8<2>(p.gamma + c0, n, gm);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) gm[j] *= fmaf(f[u][j], r0, f[u][j] * lo);
+        for (int j = 0; j < 8; ++j) {
+            const float s = f[u][j] * up;
+            gm[j] *= fmaf(s, r0, s * lo);
+        }
         if constexpr (FMT < 0) {
             if (row < p.rows && n > 0)
                 mx_store8<TO>(reinterpret_cast<typename MxElem<TO>::type*>(p.out) + row * p.C + c0, n, gm);

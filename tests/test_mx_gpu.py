@@ -606,3 +606,37 @@ def test_gate_in_fp32(dev, act, dtype):
         for a in (1.0, -3.0):
             y = ops().gated(torch.stack([torch.full_like(b, a), b], 1).to(dev), act=act, out_dtype=torch.float32).view(-1)
             within(y, a * O.gate(b.double(), act), rel, torch.float32)
+
+
+# ----------------------------------------------------------------------------- the norm at fp32's ends, and what its results hold
+
+
+@pytest.mark.parametrize("fmt", [None, "mxfp8"])
+@pytest.mark.parametrize("dtype,scale", [("f32", 1e-44), ("f32", 1e-42), ("f32", 1e-40), ("f32", 1e-38), ("f32", 1e-30), ("f32", 1e-28), ("f32", 1e28), ("f32", 1e30),
+                                         ("f32", 3.3e38), ("bf16", 1e-40), ("bf16", 1e-38), ("bf16", 3.3e38)])
+def test_rmsnorm_at_the_ends_of_fp32(dev, dtype, scale, fmt):
+    """Rows of subnormals, whose reciprocal root no fp32 number holds, and rows next to the largest number, whose one is
+    subnormal (eps 0): the formula's result, to the ordinary bound, and s as it is."""
+    x = (torch.randn(6, 700, generator=torch.Generator().manual_seed(4)).double().clamp(-1, 1) * scale).to(TYPES[dtype])
+    x[1, 50:] = 0.0
+    gamma = 1 + 0.2 * torch.randn(700, generator=torch.Generator().manual_seed(5))
+    y, s = ops().rmsnorm(x.to(dev), gamma.to(dev), 0.0, res=torch.zeros_like(x).to(dev), fmt=fmt)
+    assert torch.equal(s.cpu(), x)
+    want = O.rmsnorm(x.double(), gamma.double(), 0.0)
+    if fmt is None:
+        within(y, want, 4 * 2.0 ** -24, TYPES[dtype])
+    else:
+        assert O.held_within(ops().mx_dequantize(y).double().cpu(), want, 4 * 2.0 ** -24, fmt)
+
+
+@pytest.mark.parametrize("rows,c,dtype", [(64, 33, "f32"), (64, 1027, "f32"), (16, 5120, "f32"), (16, 5120, "bf16"), (4, 16384, "f16")])
+def test_rmsnorm_in_fp32(dev, rows, c, dtype):
+    """fp32 results.  s is the fp32 sum that the formula states; squares, their sum and the reciprocal root in fp64 and the latter
+    as two fp32 numbers leave 2^-40; the value times the root is rounded once and its product with gamma once: 2 x 2^-24.  (A
+    root in fp32 would be off by up to half a step more, for all values of its row.)"""
+    x, r = data(rows, c, c, dtype), data(rows, c, c + 1, dtype)
+    gamma = 1 + 0.2 * torch.randn(c, generator=torch.Generator().manual_seed(c))
+    y, _ = ops().rmsnorm(x.to(dev), gamma.to(dev), 1e-5, res=r.to(dev), out_dtype=torch.float32)
+    want = O.rmsnorm((x.float() + r.float()).double(), gamma.double(), float(torch.tensor(1e-5)))
+    off = (y.double().cpu() - want).abs()
+    assert bool((off <= want.abs() * 2.1 * 2.0 ** -24).all()), float((off / want.abs()).max()) * 2 ** 24
