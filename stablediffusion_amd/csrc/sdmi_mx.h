@@ -16,6 +16,9 @@ constexpr int MX_BLOCK = 32, MX_KSTEP = 128;
 __host__ __device__ __forceinline__ int64_t mx_ksteps(int64_t K) { return (K + MX_KSTEP - 1) / MX_KSTEP; }
 __host__ __device__ __forceinline__ int64_t mx_row_bytes(int64_t K, int fmt) { return mx_ksteps(K) * (fmt == SDMI_MX_FP8 ? 128 : 64); }
 
+// A launch holds fewer than 2^32 threads: the most workgroups of `threads` that it may have.
+constexpr int64_t mx_grid_blocks(int threads) { return (((int64_t)1 << 32) - 1) / threads; }
+
 // Source types of the element-wise kernels: 0 bf16, 1 f16, 2 fp32 (sdmi_dtype mapped by mx_src_type on the host).
 static inline int mx_src_type(int32_t dtype) {
     return dtype == SDMI_DTYPE_BF16 ? 0 : dtype == SDMI_DTYPE_F16 ? 1 : dtype == SDMI_DTYPE_F32 ? 2 : -1;

@@ -14,6 +14,7 @@ constexpr int EL_ROWS = 16;
 struct MxElemArgs {
     const void* x;
     int64_t ldx, rows, K;      // gated: K = the width of one half, the gate starts at column K
+    int64_t row0;              // the launch's first row
     void* out;                 // FMT none: [rows][ld_out] of the source's type or the given one
     int64_t ld_out;
     unsigned char* codes;
@@ -27,7 +28,7 @@ __global__ __launch_bounds__(256) void sdmi_mx_elem_kernel(MxElemArgs p) {
     typedef typename MxElem<T>::type E;
     const unsigned tile_r = blockIdx.x / p.ktiles, tile_k = blockIdx.x - tile_r * p.ktiles;
     const int lane = threadIdx.x & 63, sub = threadIdx.x & 15;
-    const int64_t row = (int64_t)tile_r * EL_ROWS + (threadIdx.x >> 4);
+    const int64_t row = p.row0 + (int64_t)tile_r * EL_ROWS + (threadIdx.x >> 4);
     const int64_t nsteps = mx_ksteps(p.K);
     const int64_t src_row = row < p.rows ? row : p.rows - 1;     // (the 16 lanes of a row past the end work on the last one and store nothing)
     const E* const xr = reinterpret_cast<const E*>(p.x) + src_row * p.ldx;
@@ -75,7 +76,7 @@ template <int FMT, int TO, int EL_STEPS>
 __global__ __launch_bounds__(256) void sdmi_mx_dequantise_kernel(MxElemArgs p) {
     const unsigned tile_r = blockIdx.x / p.ktiles, tile_k = blockIdx.x - tile_r * p.ktiles;
     const int sub = threadIdx.x & 15;
-    const int64_t row = (int64_t)tile_r * EL_ROWS + (threadIdx.x >> 4), nsteps = mx_ksteps(p.K);
+    const int64_t row = p.row0 + (int64_t)tile_r * EL_ROWS + (threadIdx.x >> 4), nsteps = mx_ksteps(p.K);
     if (row >= p.rows) return;
     uint2 c[EL_STEPS];
     unsigned char sc[EL_STEPS];
@@ -124,7 +125,7 @@ struct MxNormArgs {
     void* out;
     unsigned char* codes;
     unsigned char* scales;
-    int64_t ldx, ld_res, rows, C;
+    int64_t ldx, ld_res, rows, C, row0;      // row0: the launch's first row
     double inv_c;
     float eps;
 };
@@ -141,7 +142,7 @@ __global__ __launch_bounds__(256) void sdmi_rmsnorm_kernel(MxNormArgs p) {
     constexpr unsigned RUN = 8;
     unsigned block = blockIdx.x;
     if (block < gridDim.x / (8 * RUN) * (8 * RUN)) block = block / (8 * RUN) * (8 * RUN) + (block & 7) * RUN + block % (8 * RUN) / 8;
-    const int64_t row = (int64_t)block * RPB + r, srow = row < p.rows ? row : p.rows - 1;
+    const int64_t row = p.row0 + (int64_t)block * RPB + r, srow = row < p.rows ? row : p.rows - 1;
     const E* const xr = reinterpret_cast<const E*>(p.x) + srow * p.ldx;
     float f[U][8], q[U][8];
 #pragma unroll
@@ -230,30 +231,35 @@ extern "C" int64_t sdmi_mx_codes_bytes(int64_t rows, int64_t K, int32_t fmt) {
 }
 extern "C" int64_t sdmi_mx_scales_bytes(int64_t rows, int64_t K) { return rows < 0 || K <= 0 ? -1 : rows * mx_ksteps(K) * 4; }
 
-// The tiles of a launch and the k-steps of each; false: more than a grid holds.
-struct ElemGrid { unsigned blocks; int steps; };
-static bool elem_grid(int64_t rows, int64_t K, MxElemArgs* a, ElemGrid* g) {
+// The k-steps of a tile, and a launch for every `rows` rows: all of them but where the tiles are more than a grid holds.
+struct ElemGrid { int64_t rows; int steps; };
+static ElemGrid elem_grid(int64_t rows, int64_t K, MxElemArgs* a) {
     const int64_t rt = (rows + EL_ROWS - 1) / EL_ROWS, ks = mx_ksteps(K);
-    g->steps = rt * ((ks + 3) / 4) >= 1024 ? 4 : 1;
-    a->ktiles = (unsigned)((ks + g->steps - 1) / g->steps);
-    g->blocks = (unsigned)(rt * a->ktiles);
-    return rt * a->ktiles < ((int64_t)1 << 31);
+    const int steps = rt * ((ks + 3) / 4) >= 1024 ? 4 : 1;
+    a->ktiles = (unsigned)((ks + steps - 1) / steps);
+    return {mx_grid_blocks(256) / a->ktiles * EL_ROWS, steps};
+}
+template <class F> static int elem_rows(MxElemArgs a, const ElemGrid& g, F&& launch) {
+    for (; a.row0 < a.rows; a.row0 += g.rows) {
+        const int64_t rows = a.rows - a.row0 < g.rows ? a.rows - a.row0 : g.rows;
+        launch(a, (unsigned)((rows + EL_ROWS - 1) / EL_ROWS * a.ktiles));
+        SDMI_CHECK_LAUNCH();
+    }
+    return SDMI_OK;
 }
 
-template <int T, int OP, int FMT, int TO> static void elem_steps(const MxElemArgs& a, const ElemGrid& g, hipStream_t st) {
-    if (g.steps == 4) sdmi_mx_elem_kernel<T, OP, FMT, TO, 4><<<g.blocks, 256, 0, st>>>(a);
-    else sdmi_mx_elem_kernel<T, OP, FMT, TO, 1><<<g.blocks, 256, 0, st>>>(a);
+template <int T, int OP, int FMT, int TO> static int elem_steps(const MxElemArgs& a, const ElemGrid& g, hipStream_t st) {
+    return elem_rows(a, g, [&](const MxElemArgs& b, unsigned blocks) {
+        if (g.steps == 4) sdmi_mx_elem_kernel<T, OP, FMT, TO, 4><<<blocks, 256, 0, st>>>(b);
+        else sdmi_mx_elem_kernel<T, OP, FMT, TO, 1><<<blocks, 256, 0, st>>>(b);
+    });
 }
 template <int T, int OP>
 static int elem_launch(const MxElemArgs& a, int fmt, int to, const ElemGrid& g, hipStream_t st) {
-    if (fmt == SDMI_MX_FP8) elem_steps<T, OP, SDMI_MX_FP8, 0>(a, g, st);
-    else if (fmt == SDMI_MX_FP4) elem_steps<T, OP, SDMI_MX_FP4, 0>(a, g, st);
-    else if constexpr (OP == 0) return SDMI_ERR_BAD_ARG;
-    else if (to == 0) elem_steps<T, OP, -1, 0>(a, g, st);
-    else if (to == 1) elem_steps<T, OP, -1, 1>(a, g, st);
-    else elem_steps<T, OP, -1, 2>(a, g, st);
-    SDMI_CHECK_LAUNCH();
-    return SDMI_OK;
+    if (fmt == SDMI_MX_FP8) return elem_steps<T, OP, SDMI_MX_FP8, 0>(a, g, st);
+    if (fmt == SDMI_MX_FP4) return elem_steps<T, OP, SDMI_MX_FP4, 0>(a, g, st);
+    if constexpr (OP == 0) return SDMI_ERR_BAD_ARG;
+    else return to == 0 ? elem_steps<T, OP, -1, 0>(a, g, st) : to == 1 ? elem_steps<T, OP, -1, 1>(a, g, st) : elem_steps<T, OP, -1, 2>(a, g, st);
 }
 
 extern "C" int sdmi_mx_quantize(const void* x, int64_t ldx, int64_t rows, int64_t K, int32_t dtype, void* codes, void* scales,
@@ -264,8 +270,7 @@ extern "C" int sdmi_mx_quantize(const void* x, int64_t ldx, int64_t rows, int64_
     if (rows == 0) return SDMI_OK;
     MxElemArgs a = {};
     a.x = x; a.ldx = ldx; a.rows = rows; a.K = K; a.codes = (unsigned char*)codes; a.scales = (unsigned char*)scales;
-    ElemGrid g;
-    if (!elem_grid(rows, K, &a, &g)) return SDMI_ERR_BAD_ARG;
+    const ElemGrid g = elem_grid(rows, K, &a);
     hipStream_t st = (hipStream_t)stream;
     return t == 0 ? elem_launch<0, 0>(a, fmt, 0, g, st) : t == 1 ? elem_launch<1, 0>(a, fmt, 0, g, st) : elem_launch<2, 0>(a, fmt, 0, g, st);
 }
@@ -280,8 +285,7 @@ extern "C" int sdmi_gated(const void* x, int64_t ldx, int64_t rows, int64_t inne
     MxElemArgs a = {};
     a.x = x; a.ldx = ldx; a.rows = rows; a.K = inner; a.codes = (unsigned char*)out; a.scales = (unsigned char*)scales;
     a.out = out; a.ld_out = inner;
-    ElemGrid g;
-    if (!elem_grid(rows, inner, &a, &g)) return SDMI_ERR_BAD_ARG;
+    const ElemGrid g = elem_grid(rows, inner, &a);
     hipStream_t st = (hipStream_t)stream;
     if (act == 0)
         return t == 0 ? elem_launch<0, 1>(a, fmt, to, g, st) : t == 1 ? elem_launch<1, 1>(a, fmt, to, g, st) : elem_launch<2, 1>(a, fmt, to, g, st);
@@ -296,14 +300,22 @@ extern "C" int sdmi_mx_dequantize(const void* codes, const void* scales, int64_t
     if (rows == 0) return SDMI_OK;
     MxElemArgs a = {};
     a.rows = rows; a.K = K; a.codes = (unsigned char*)codes; a.scales = (unsigned char*)scales; a.out = out; a.ld_out = ld_out;
-    ElemGrid g;
-    if (!elem_grid(rows, K, &a, &g)) return SDMI_ERR_BAD_ARG;
+    const ElemGrid g = elem_grid(rows, K, &a);
     hipStream_t st = (hipStream_t)stream;
-#define SDMI_DQ(F, O) do { if (g.steps == 4) sdmi_mx_dequantise_kernel<F, O, 4><<<g.blocks, 256, 0, st>>>(a); else sdmi_mx_dequantise_kernel<F, O, 1><<<g.blocks, 256, 0, st>>>(a); } while (0)
-    if (fmt == SDMI_MX_FP8) { if (to == 0) SDMI_DQ(SDMI_MX_FP8, 0); else if (to == 1) SDMI_DQ(SDMI_MX_FP8, 1); else SDMI_DQ(SDMI_MX_FP8, 2); }
-    else { if (to == 0) SDMI_DQ(SDMI_MX_FP4, 0); else if (to == 1) SDMI_DQ(SDMI_MX_FP4, 1); else SDMI_DQ(SDMI_MX_FP4, 2); }
+#define SDMI_DQ(F, O) elem_rows(a, g, [&](const MxElemArgs& b, unsigned blocks) { \
+        if (g.steps == 4) sdmi_mx_dequantise_kernel<F, O, 4><<<blocks, 256, 0, st>>>(b); else sdmi_mx_dequantise_kernel<F, O, 1><<<blocks, 256, 0, st>>>(b); })
+    if (fmt == SDMI_MX_FP8) return to == 0 ? SDMI_DQ(SDMI_MX_FP8, 0) : to == 1 ? SDMI_DQ(SDMI_MX_FP8, 1) : SDMI_DQ(SDMI_MX_FP8, 2);
+    return to == 0 ? SDMI_DQ(SDMI_MX_FP4, 0) : to == 1 ? SDMI_DQ(SDMI_MX_FP4, 1) : SDMI_DQ(SDMI_MX_FP4, 2);
 #undef SDMI_DQ
-    SDMI_CHECK_LAUNCH();
+}
+
+template <int T, int FMT, int TO, int TPR, int U> static int norm_rows(MxNormArgs a, hipStream_t st) {
+    constexpr int RPB = 256 / TPR;
+    for (; a.row0 < a.rows; a.row0 += mx_grid_blocks(256) * RPB) {             // (one launch but for more rows than a grid holds)
+        const int64_t blocks = (a.rows - a.row0 + RPB - 1) / RPB;
+        sdmi_rmsnorm_kernel<T, FMT, TO, TPR, U><<<(unsigned)(blocks < mx_grid_blocks(256) ? blocks : mx_grid_blocks(256)), 256, 0, st>>>(a);
+        SDMI_CHECK_LAUNCH();
+    }
     return SDMI_OK;
 }
 
@@ -312,22 +324,18 @@ static int norm_launch(const MxNormArgs& a, hipStream_t st) {
     // As few threads a row as hold it in one chunk of 8 values each, and from 2048 values on 256 threads with as many chunks as
     // the row needs and no more: an empty chunk costs registers and instructions (16384 x 5120: 256 x 3 120 us, 256 x 4 143,
     // 128 x 5 148, 512 x 2 127, 64 x 10 208; 32768 x 1024: 128 x 1 47 us, 64 x 2 50, 256 x 1 58).
-#define SDMI_NORM(TPR, U) sdmi_rmsnorm_kernel<T, FMT, TO, TPR, U><<<(unsigned)((a.rows + 256 / TPR - 1) / (256 / TPR)), 256, 0, st>>>(a)
-    if (a.C <= 512) SDMI_NORM(64, 1);
-    else if (a.C <= 1024) SDMI_NORM(128, 1);
-    else switch ((a.C + 2047) / 2048) {
-        case 1: SDMI_NORM(256, 1); break;
-        case 2: SDMI_NORM(256, 2); break;
-        case 3: SDMI_NORM(256, 3); break;
-        case 4: SDMI_NORM(256, 4); break;
-        case 5: SDMI_NORM(256, 5); break;
-        case 6: SDMI_NORM(256, 6); break;
-        case 7: SDMI_NORM(256, 7); break;
-        default: SDMI_NORM(256, 8);
+    if (a.C <= 512) return norm_rows<T, FMT, TO, 64, 1>(a, st);
+    if (a.C <= 1024) return norm_rows<T, FMT, TO, 128, 1>(a, st);
+    switch ((a.C + 2047) / 2048) {
+        case 1: return norm_rows<T, FMT, TO, 256, 1>(a, st);
+        case 2: return norm_rows<T, FMT, TO, 256, 2>(a, st);
+        case 3: return norm_rows<T, FMT, TO, 256, 3>(a, st);
+        case 4: return norm_rows<T, FMT, TO, 256, 4>(a, st);
+        case 5: return norm_rows<T, FMT, TO, 256, 5>(a, st);
+        case 6: return norm_rows<T, FMT, TO, 256, 6>(a, st);
+        case 7: return norm_rows<T, FMT, TO, 256, 7>(a, st);
+        default: return norm_rows<T, FMT, TO, 256, 8>(a, st);
     }
-#undef SDMI_NORM
-    SDMI_CHECK_LAUNCH();
-    return SDMI_OK;
 }
 
 template <int T> static int norm_type(const MxNormArgs& a, int fmt, int to, hipStream_t st) {

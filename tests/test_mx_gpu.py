@@ -640,3 +640,29 @@ def test_rmsnorm_in_fp32(dev, rows, c, dtype):
     want = O.rmsnorm((x.float() + r.float()).double(), gamma.double(), float(torch.tensor(1e-5)))
     off = (y.double().cpu() - want).abs()
     assert bool((off <= want.abs() * 2.1 * 2.0 ** -24).all()), float((off / want.abs()).max()) * 2 ** 24
+
+
+# ----------------------------------------------------------------------------- more rows than a launch holds
+
+
+@pytest.mark.parametrize("op", ["quantise", "gate", "norm"])
+def test_more_rows_than_a_launch_holds(dev, op):
+    """A launch has fewer than 2^32 threads, 2^24 - 1 workgroups of 256: 16 rows each of the element-wise operators, 4 of the norm's
+    narrow rows.  Rows on both sides of that border and the last ones against the same rows alone, nothing elsewhere."""
+    o = ops()
+    border = ((1 << 24) - 1) * (4 if op == "norm" else 16)
+    rows, width = border + 1003, 1 if op == "quantise" else 2
+    windows = [(0, 50), (border - 70, border + 70), (rows - 300, rows)]
+    parts = [data(b - a, width, i + 1, loud=False).to(dev) for i, (a, b) in enumerate(windows)]
+    x = torch.zeros(rows, width, dtype=torch.bfloat16, device=dev)
+    for (a, b), part in zip(windows, parts):
+        x[a:b] = part
+    gamma = torch.ones(width, device=dev)
+    run = {"quantise": lambda t: o.mx_dequantize(o.mx_quantize(t, "mxfp4"), torch.bfloat16), "gate": lambda t: o.gated(t),
+           "norm": lambda t: o.rmsnorm(t, gamma, 1.0, res=t)}[op]
+    got, want = run(x), [run(part) for part in parts]
+    for i in range(2 if op == "norm" else 1):
+        y, alone = (got[i], [w[i] for w in want]) if op == "norm" else (got, want)
+        for (a, b), w in zip(windows, alone):
+            assert torch.equal(y[a:b], w), (i, a)
+        assert int(torch.count_nonzero(y)) == sum(int(torch.count_nonzero(w)) for w in alone), i
