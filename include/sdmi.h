@@ -419,7 +419,8 @@ int sdmi_image_to_u8(const float* x, uint8_t* out, int32_t nb, int32_t C, int64_
  * Format (OCP Microscaling v1.0): blocks of 32 consecutive values of a row share a scale 2^(byte - 127); elements are e4m3
  * (SDMI_MX_FP8, largest 448) or e2m1 (SDMI_MX_FP4, largest 6).  byte = max(0, floor(log2 max|x|) - emax + 127) with emax 8
  * or 2; an element is x / scale rounded to nearest even and saturated.  A block that holds a NaN or an infinity becomes
- * NaN as a whole (byte 255).  K is any positive number up to 2^24; the last block is filled with zeros.
+ * NaN as a whole (byte 255).  K is any positive number up to 2^24, rows
+ * fewer than 2^31, N of weights up to 2^24; the last block is filled with zeros.
  *   activations: codes in planes of 64 bytes a row: [Kp / 64][rows][64] (FP8) or [Kp / 128][rows][64] (FP4, even k in the low nibble),
  *       Kp = K rounded up to 128; scales [Kp / 128][rows][4 bytes] (the four blocks of a row's 128 values).  Sizes: sdmi_mx_codes_bytes,
  *       sdmi_mx_scales_bytes (-1 for sizes that are refused).

@@ -16,6 +16,10 @@ constexpr int MX_BLOCK = 32, MX_KSTEP = 128;
 __host__ __device__ __forceinline__ int64_t mx_ksteps(int64_t K) { return (K + MX_KSTEP - 1) / MX_KSTEP; }
 __host__ __device__ __forceinline__ int64_t mx_row_bytes(int64_t K, int fmt) { return mx_ksteps(K) * (fmt == SDMI_MX_FP8 ? 128 : 64); }
 
+// What the operators take, and what their size queries answer for: -1 beyond.
+constexpr int64_t MX_MAX_DIM = (int64_t)1 << 24, MX_MAX_ROWS = ((int64_t)1 << 31) - 1;      // K (and N of weights); rows
+static inline bool mx_sizes_ok(int64_t rows, int64_t K) { return rows >= 0 && rows <= MX_MAX_ROWS && K > 0 && K <= MX_MAX_DIM; }
+
 // A launch holds fewer than 2^32 threads: the most workgroups of `threads` that it may have.
 constexpr int64_t mx_grid_blocks(int threads) { return (((int64_t)1 << 32) - 1) / threads; }
 

@@ -224,12 +224,11 @@ __global__ __launch_bounds__(256) void sdmi_rmsnorm_kernel(MxNormArgs p) {
 // ---- host side ---------------------------------------------------------------------------------------------------------
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 static bool fmt_ok(int32_t fmt) { return fmt == SDMI_MX_FP8 || fmt == SDMI_MX_FP4; }
-constexpr int64_t MX_MAX_K = (int64_t)1 << 24, MX_MAX_ROWS = ((int64_t)1 << 31) - 1;
 
 extern "C" int64_t sdmi_mx_codes_bytes(int64_t rows, int64_t K, int32_t fmt) {
-    return rows < 0 || K <= 0 || !fmt_ok(fmt) ? -1 : rows * mx_row_bytes(K, fmt);
+    return !mx_sizes_ok(rows, K) || !fmt_ok(fmt) ? -1 : rows * mx_row_bytes(K, fmt);
 }
-extern "C" int64_t sdmi_mx_scales_bytes(int64_t rows, int64_t K) { return rows < 0 || K <= 0 ? -1 : rows * mx_ksteps(K) * 4; }
+extern "C" int64_t sdmi_mx_scales_bytes(int64_t rows, int64_t K) { return !mx_sizes_ok(rows, K) ? -1 : rows * mx_ksteps(K) * 4; }
 
 // The k-steps of a tile, and a launch for every `rows` rows: all of them but where the tiles are more than a grid holds.
 struct ElemGrid { int64_t rows; int steps; };
@@ -265,7 +264,7 @@ static int elem_launch(const MxElemArgs& a, int fmt, int to, const ElemGrid& g, 
 extern "C" int sdmi_mx_quantize(const void* x, int64_t ldx, int64_t rows, int64_t K, int32_t dtype, void* codes, void* scales,
                                 int32_t fmt, void* stream) {
     const int t = mx_src_type(dtype);
-    if (!x || !codes || !scales || t < 0 || !fmt_ok(fmt) || rows < 0 || K <= 0 || K > MX_MAX_K || ldx < K || rows > MX_MAX_ROWS) return SDMI_ERR_BAD_ARG;
+    if (!x || !codes || !scales || t < 0 || !fmt_ok(fmt) || !mx_sizes_ok(rows, K) || ldx < K) return SDMI_ERR_BAD_ARG;
     if (!aligned16(codes) || !aligned16(scales)) return SDMI_ERR_ALIGNMENT;
     if (rows == 0) return SDMI_OK;
     MxElemArgs a = {};
@@ -279,7 +278,7 @@ extern "C" int sdmi_gated(const void* x, int64_t ldx, int64_t rows, int64_t inne
                           int32_t out_dtype, void* scales, int32_t fmt, void* stream) {
     const int t = mx_src_type(dtype), to = fmt == SDMI_MX_NONE ? mx_src_type(out_dtype) : 0;
     if (!x || !out || t < 0 || to < 0 || (act != 0 && act != 1) || (fmt != SDMI_MX_NONE && (!fmt_ok(fmt) || !scales)) ||
-        rows < 0 || inner <= 0 || inner > MX_MAX_K || ldx < 2 * inner || rows > MX_MAX_ROWS) return SDMI_ERR_BAD_ARG;
+        !mx_sizes_ok(rows, inner) || ldx < 2 * inner) return SDMI_ERR_BAD_ARG;
     if (fmt != SDMI_MX_NONE && (!aligned16(out) || !aligned16(scales))) return SDMI_ERR_ALIGNMENT;
     if (rows == 0) return SDMI_OK;
     MxElemArgs a = {};
@@ -295,7 +294,7 @@ extern "C" int sdmi_gated(const void* x, int64_t ldx, int64_t rows, int64_t inne
 extern "C" int sdmi_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t K, int32_t fmt, void* out,
                                   int64_t ld_out, int32_t out_dtype, void* stream) {
     const int to = mx_src_type(out_dtype);
-    if (!codes || !scales || !out || to < 0 || !fmt_ok(fmt) || rows < 0 || K <= 0 || K > MX_MAX_K || ld_out < K || rows > MX_MAX_ROWS) return SDMI_ERR_BAD_ARG;
+    if (!codes || !scales || !out || to < 0 || !fmt_ok(fmt) || !mx_sizes_ok(rows, K) || ld_out < K) return SDMI_ERR_BAD_ARG;
     if (!aligned16(codes) || !aligned16(scales)) return SDMI_ERR_ALIGNMENT;
     if (rows == 0) return SDMI_OK;
     MxElemArgs a = {};
@@ -348,8 +347,8 @@ extern "C" int sdmi_rmsnorm(const void* x, int64_t ldx, const void* res, int64_t
                             int64_t rows, int64_t C, int32_t dtype, void* sum_out, void* out, int32_t out_dtype, void* scales,
                             int32_t fmt, void* stream) {
     const int t = mx_src_type(dtype), to = fmt == SDMI_MX_NONE ? mx_src_type(out_dtype) : 0;
-    if (!x || !gamma || !out || t < 0 || to < 0 || (fmt != SDMI_MX_NONE && (!fmt_ok(fmt) || !scales)) || rows < 0 || C <= 0 ||
-        C > SDMI_RMSNORM_MAX_C || ldx < C || (res && (ld_res < C || !sum_out)) || rows > MX_MAX_ROWS || !(eps >= 0.0f)) return SDMI_ERR_BAD_ARG;
+    if (!x || !gamma || !out || t < 0 || to < 0 || (fmt != SDMI_MX_NONE && (!fmt_ok(fmt) || !scales)) || !mx_sizes_ok(rows, C) ||
+        C > SDMI_RMSNORM_MAX_C || ldx < C || (res && (ld_res < C || !sum_out)) || !(eps >= 0.0f)) return SDMI_ERR_BAD_ARG;
     if (!aligned16(gamma) || (fmt != SDMI_MX_NONE && (!aligned16(out) || !aligned16(scales)))) return SDMI_ERR_ALIGNMENT;
     if (rows == 0) return SDMI_OK;
     MxNormArgs a = {};

@@ -657,17 +657,19 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void sdmi_mx_tiled_kernel(MxGemm
 
 // ---- host side ---------------------------------------------------------------------------------------------------------
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-constexpr int64_t MX_MAX_DIM = (int64_t)1 << 24;
 
-extern "C" int64_t sdmi_mx_weight_codes_bytes(int64_t N, int64_t K) { return N <= 0 || K <= 0 ? -1 : (N + 63) / 64 * mx_ksteps(K) * 4096; }
-extern "C" int64_t sdmi_mx_weight_scales_bytes(int64_t N, int64_t K) { return N <= 0 || K <= 0 ? -1 : (N + 63) / 64 * mx_ksteps(K) * 256; }
+// (the packing kernel's threads, one for a block of 32, in one launch)
+static bool mx_weight_ok(int64_t N, int64_t K) {
+    return N > 0 && N <= MX_MAX_DIM && K > 0 && K <= MX_MAX_DIM && ((N + 63) / 64 * 64 * mx_ksteps(K) * 4 + 255) / 256 <= mx_grid_blocks(256);
+}
+extern "C" int64_t sdmi_mx_weight_codes_bytes(int64_t N, int64_t K) { return mx_weight_ok(N, K) ? (N + 63) / 64 * mx_ksteps(K) * 4096 : -1; }
+extern "C" int64_t sdmi_mx_weight_scales_bytes(int64_t N, int64_t K) { return mx_weight_ok(N, K) ? (N + 63) / 64 * mx_ksteps(K) * 256 : -1; }
 
 extern "C" int sdmi_mx_pack_linear(const void* w, int64_t ldw, int64_t N, int64_t K, int32_t dtype, void* codes, void* scales, void* stream) {
     const int t = mx_src_type(dtype);
-    if (!w || !codes || !scales || t < 0 || N <= 0 || K <= 0 || N > MX_MAX_DIM || K > MX_MAX_DIM || ldw < K) return SDMI_ERR_BAD_ARG;
+    if (!w || !codes || !scales || t < 0 || !mx_weight_ok(N, K) || ldw < K) return SDMI_ERR_BAD_ARG;
     if (!aligned16(codes) || !aligned16(scales)) return SDMI_ERR_ALIGNMENT;
     const int64_t n = (N + 63) / 64 * 64 * mx_ksteps(K) * 4, blocks = (n + 255) / 256;
-    if (blocks >= ((int64_t)1 << 31)) return SDMI_ERR_BAD_ARG;
     hipStream_t st = (hipStream_t)stream;
     unsigned char *c = (unsigned char*)codes, *s = (unsigned char*)scales;
     if (t == 0) sdmi_mx_pack_kernel<0><<<(unsigned)blocks, 256, 0, st>>>((const unsigned short*)w, ldw, N, K, c, s);
@@ -680,7 +682,7 @@ extern "C" int sdmi_mx_pack_linear(const void* w, int64_t ldw, int64_t N, int64_
 static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
 static bool mx_args_ok(const sdmi_mx_gemm_args* a) {
-    if (!a || a->M < 0 || a->N <= 0 || a->K <= 0 || a->M >= ((int64_t)1 << 31) || a->N > MX_MAX_DIM || a->K > MX_MAX_DIM) return false;
+    if (!a || !mx_sizes_ok(a->M, a->K) || !mx_weight_ok(a->N, a->K)) return false;
     if ((a->fmt != SDMI_MX_FP8 && a->fmt != SDMI_MX_FP4) || a->algo < 0 || a->algo > SDMI_MX_ALGOS) return false;
     return !a->x || (mx_src_type(a->x_dtype) >= 0 && a->ldx >= a->K);
 }
@@ -727,14 +729,20 @@ static double mx_cost(const sdmi_mx_gemm_args* a, int kind) {
     const double units = (double)((mx_ksteps(a->K) + c.unit - 1) / c.unit);
     return us.fixed + us.first * units + (double)(mx_rounds(a, kind) - 1) * (us.round + us.more * units);
 }
-static MxKind mx_kind(const sdmi_mx_gemm_args* a) {
-    if (a->algo) return (MxKind)(a->algo - 1);
-    int best = MX_T256x256;
-    double least = mx_cost(a, best);
-    for (int i = MX_KINDS - 2; i >= 0; --i) {
-        if (MX_COST[i].unit > 1 && a->M > 65535 * (int64_t)MX_COST[i].rows) continue;      // the direct kernels' grid
+// Whether a kernel's workgroups fit a launch: rows go along y in the direct kernels (512 threads), all tiles along x in the tiled
+// ones (two wave rows for every 64 columns).
+static bool mx_fits(const sdmi_mx_gemm_args* a, int kind) {
+    const MxCost& c = MX_COST[kind];
+    const int64_t ny = (a->M + c.rows - 1) / c.rows, nx = (a->N + c.cols - 1) / c.cols;
+    return c.unit > 1 ? ny <= 65535 && nx <= mx_grid_blocks(512) : ny * nx <= mx_grid_blocks(2 * c.cols);
+}
+static MxKind mx_kind(const sdmi_mx_gemm_args* a) {                              // MX_KINDS: none
+    if (a->algo) return mx_fits(a, a->algo - 1) ? (MxKind)(a->algo - 1) : MX_KINDS;
+    int best = MX_KINDS;
+    double least = 0.0;
+    for (int i = MX_KINDS - 1; i >= 0; --i) {
         const double cost = mx_cost(a, i);
-        if (cost < least) { best = i; least = cost; }
+        if ((best == MX_KINDS || cost < least) && mx_fits(a, i)) { best = i; least = cost; }
     }
     return (MxKind)best;
 }
@@ -759,14 +767,24 @@ static MxFused mx_fused(const sdmi_mx_gemm_args* a) {
     return r16 * c64 <= 512 ? MX_FUSED16x64 : MX_APART;
 }
 
+// How a product runs and the workspace it needs; false: not at all, said before anything of it is launched.
+struct MxPlan { MxFused fused; MxKind kind; int64_t workspace; };
+static bool mx_plan(const sdmi_mx_gemm_args* a, MxPlan* p) {
+    if (!mx_args_ok(a)) return false;
+    p->fused = mx_fused(a);
+    p->kind = p->fused ? MX_KINDS : mx_kind(a);
+    p->workspace = !a->x || a->M == 0 || p->fused ? 0 : up256(a->M * mx_row_bytes(a->K, a->fmt)) + up256(a->M * mx_ksteps(a->K) * 4);
+    return p->fused || p->kind != MX_KINDS;
+}
+
 extern "C" int64_t sdmi_mx_gemm_workspace_bytes(const sdmi_mx_gemm_args* a) {
-    if (!mx_args_ok(a)) return -1;
-    if (!a->x || a->M == 0 || mx_fused(a)) return 0;
-    return up256(a->M * mx_row_bytes(a->K, a->fmt)) + up256(a->M * mx_ksteps(a->K) * 4);
+    MxPlan p;
+    return mx_plan(a, &p) ? p.workspace : -1;
 }
 
 template <int FMT, int BM, int WGM, int WGN, int ST> static int tiled_launch(const MxGemmDev& d, hipStream_t st) {
     typedef MxTile<FMT, BM, WGM, WGN, ST> T;
+    static_assert(T::THREADS == 2 * T::BN, "mx_fits");
     static SdmiPerDeviceOnce once;
     const auto kernel = sdmi_mx_tiled_kernel<FMT, BM, WGM, WGN, ST>;
     if (T::LDS > 65536) {
@@ -774,7 +792,6 @@ template <int FMT, int BM, int WGM, int WGN, int ST> static int tiled_launch(con
         if (r != SDMI_OK) return r;
     }
     const int64_t tiles = (d.M + BM - 1) / BM * ((d.N + T::BN - 1) / T::BN);
-    if (tiles >= ((int64_t)1 << 31)) return SDMI_ERR_BAD_ARG;
     kernel<<<(unsigned)tiles, T::THREADS, T::LDS, st>>>(d);
     SDMI_CHECK_LAUNCH();
     return SDMI_OK;
@@ -783,7 +800,6 @@ template <int FMT, int BM, int WGM, int WGN, int ST> static int tiled_launch(con
 template <int FMT, int MT, int NF, int KW, int U, int SRC> static int direct_launch(const MxGemmDev& d, hipStream_t st) {
     const int sums = KW * MT * NF * 1024, codes = SRC < 0 ? 0 : (int)(d.ksteps * (d.M < 16 * MT ? d.M : 16 * MT) * (mx_row_bytes(128, FMT) + 4));
     const int64_t nx = (d.N + 63) / 64 * (4 / NF), ny = (d.M + 16 * MT - 1) / (16 * MT);
-    if (ny > 65535) return SDMI_ERR_BAD_ARG;
     if (KW * MT * NF * 1024 > 65536) {
         static SdmiPerDeviceOnce once;
         const int r = once.run([&] { return hipFuncSetAttribute(reinterpret_cast<const void*>(sdmi_mx_direct_kernel<FMT, MT, NF, KW, U, SRC>), hipFuncAttributeMaxDynamicSharedMemorySize, KW * MT * NF * 1024) == hipSuccess; });
@@ -825,18 +841,17 @@ template <int FMT> static int mx_launch(const MxGemmDev& d, MxKind kind, MxFused
 }
 
 extern "C" int sdmi_mx_gemm(const sdmi_mx_gemm_args* a, void* stream) {
-    if (!mx_args_ok(a) || !a->w_codes || !a->w_scales || !a->out || (!a->x && (!a->x_codes || !a->x_scales))) return SDMI_ERR_BAD_ARG;
+    MxPlan plan;
+    if (!mx_plan(a, &plan) || !a->w_codes || !a->w_scales || !a->out || (!a->x && (!a->x_codes || !a->x_scales))) return SDMI_ERR_BAD_ARG;
     const int type = mx_src_type(a->out_dtype);
     if (type < 0 || a->ld_out < a->N || (a->res && a->ld_res < a->N)) return SDMI_ERR_BAD_ARG;
     if (!aligned16(a->w_codes) || !aligned16(a->w_scales) || (!a->x && (!aligned16(a->x_codes) || !aligned16(a->x_scales)))) return SDMI_ERR_ALIGNMENT;
     if (a->M == 0) return SDMI_OK;
-    const int64_t need = sdmi_mx_gemm_workspace_bytes(a);
-    if (need > 0 && (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace))) return SDMI_ERR_WORKSPACE;
+    if (plan.workspace > 0 && (!a->workspace || a->workspace_bytes < plan.workspace || !aligned16(a->workspace))) return SDMI_ERR_WORKSPACE;
     MxGemmDev d = {};
     d.xc = (const unsigned char*)a->x_codes; d.xs = (const unsigned char*)a->x_scales;
-    const MxFused fused = mx_fused(a);
-    const int src = fused ? mx_src_type(a->x_dtype) : -1;
-    if (fused) {
+    const int src = plan.fused ? mx_src_type(a->x_dtype) : -1;
+    if (plan.fused) {
         d.x = a->x; d.ldx = a->ldx;
     } else if (a->x) {
         unsigned char* const ws = (unsigned char*)a->workspace;
@@ -849,5 +864,5 @@ extern "C" int sdmi_mx_gemm(const sdmi_mx_gemm_args* a, void* stream) {
     d.bias = a->bias; d.res = a->res; d.out = a->out;
     d.M = a->M; d.N = a->N; d.K = a->K; d.ksteps = mx_ksteps(a->K); d.ld_res = a->ld_res; d.ld_out = a->ld_out;
     d.type = type;
-    return a->fmt == SDMI_MX_FP8 ? mx_launch<SDMI_MX_FP8>(d, mx_kind(a), fused, src, (hipStream_t)stream) : mx_launch<SDMI_MX_FP4>(d, mx_kind(a), fused, src, (hipStream_t)stream);
+    return a->fmt == SDMI_MX_FP8 ? mx_launch<SDMI_MX_FP8>(d, plan.kind, plan.fused, src, (hipStream_t)stream) : mx_launch<SDMI_MX_FP4>(d, plan.kind, plan.fused, src, (hipStream_t)stream);
 }

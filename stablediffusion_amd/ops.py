@@ -1029,8 +1029,10 @@ def pack_linear_mx(weight, bias=None):
     if b is not None and b.device != w.device:
         raise hip.SdmiError(f"pack_linear_mx: bias is on {b.device}, the weight on {w.device}")
     lib = hip.lib()
-    pw = PackedMxWeight(torch.empty(lib.sdmi_mx_weight_codes_bytes(n, k), dtype=torch.uint8, device=w.device),
-                        torch.empty(lib.sdmi_mx_weight_scales_bytes(n, k), dtype=torch.uint8, device=w.device), b, n, k)
+    codes, scales = lib.sdmi_mx_weight_codes_bytes(n, k), lib.sdmi_mx_weight_scales_bytes(n, k)
+    if codes < 0:
+        raise hip.SdmiError(f"pack_linear_mx: {n} x {k} is larger than the operator takes (2^24 on a side)")
+    pw = PackedMxWeight(torch.empty(codes, dtype=torch.uint8, device=w.device), torch.empty(scales, dtype=torch.uint8, device=w.device), b, n, k)
     _mx_call(lib.sdmi_mx_pack_linear, "sdmi_mx_pack_linear", w.device, w.data_ptr(), ld, n, k, dt, pw.codes.data_ptr(), pw.scales.data_ptr())
     return pw
 

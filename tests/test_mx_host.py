@@ -144,3 +144,35 @@ def test_oracle_against_the_formats_own_tables(fmt):
     far = (got.abs()[..., None] - table).abs().amin(-1)
     assert float(far.max()) == 0.0
     assert bool(((got - want).abs() <= (want.abs()[..., None] - table).abs().amin(-1)).all())
+
+
+def test_sizes_beyond_the_limits(lib):
+    """The size queries give -1 for what the operators refuse, and nothing overflows on the way."""
+    assert lib.sdmi_mx_codes_bytes((1 << 31) - 1, 1 << 24, 1) == ((1 << 31) - 1) << 24 and lib.sdmi_mx_scales_bytes((1 << 31) - 1, 1) == ((1 << 31) - 1) * 4
+    for rows, k in ((1 << 31, 64), (1 << 62, 1), (4, (1 << 24) + 1), (4, (1 << 62) + 1)):
+        assert lib.sdmi_mx_codes_bytes(rows, k, 1) == lib.sdmi_mx_codes_bytes(rows, k, 2) == lib.sdmi_mx_scales_bytes(rows, k) == -1, (rows, k)
+        assert lib.sdmi_mx_quantize(P, k, rows, k, 0, P, P, 1, None) == lib.sdmi_mx_dequantize(P, P, rows, k, 1, P, k, 0, None) == BAD, (rows, k)
+    assert lib.sdmi_mx_weight_codes_bytes(1 << 24, 8064) == (1 << 18) * 63 * 4096
+    # N, K, and the threads of the packing launch (one for 32 values): 2^24 x 8192 would be 2^32
+    for n, k in (((1 << 24) + 1, 64), (64, (1 << 24) + 1), (1 << 62, 1), (1 << 24, 8192), (1 << 24, 1 << 24)):
+        assert lib.sdmi_mx_weight_codes_bytes(n, k) == lib.sdmi_mx_weight_scales_bytes(n, k) == -1, (n, k)
+        assert lib.sdmi_mx_pack_linear(P, k, n, k, 4, P, P, None) == BAD, (n, k)
+        assert lib.sdmi_mx_gemm_workspace_bytes(C.byref(_gemm(M=4, N=n, K=k, ldx=k, ld_out=n))) == -1, (n, k)
+
+
+def test_a_product_is_refused_before_anything_is_launched(lib):
+    """Pinned kernels whose grid does not hold the rows: the workspace query says so already, and the product refuses before it
+    quantises (a workspace of 0 bytes would be the first complaint otherwise)."""
+    size = lambda **kw: lib.sdmi_mx_gemm_workspace_bytes(C.byref(_gemm(N=64, K=64, **kw)))
+    call = lambda **kw: lib.sdmi_mx_gemm(C.byref(_gemm(N=64, K=64, **kw)), None)
+    for algo, rows in ((1, 16), (2, 16), (3, 32), (4, 48)):              # row tiles along y: at most 65535
+        assert size(M=65535 * rows, algo=algo) > 0 and size(M=65535 * rows + 1, algo=algo) == -1, algo
+        assert call(M=65535 * rows + 1, algo=algo) == BAD and call(M=65535 * rows, algo=algo) == WORKSPACE, algo
+    for algo, rows, threads in ((5, 64, 256), (6, 128, 256), (7, 128, 512), (8, 256, 512)):      # all tiles along x: fewer than 2^32 threads
+        most = min((2 ** 32 - 1) // threads * rows, 2 ** 31 - 1)
+        assert size(M=most, algo=algo) > 0 and call(M=most, algo=algo) == WORKSPACE, algo
+        if most < 2 ** 31 - 1:
+            assert size(M=most + 1, algo=algo) == -1 and call(M=most + 1, algo=algo) == BAD, algo
+    # left to itself the library takes a kernel that holds them, and none past the largest tiles' last full launch
+    assert size(M=65535 * 48 + 1) > 0 and size(M=2 ** 31 - 256) > 0 and size(M=2 ** 31) == -1
+    assert size(M=2 ** 31 - 1) == -1 and call(M=2 ** 31 - 1) == BAD
