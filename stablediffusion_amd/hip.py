@@ -14,6 +14,7 @@ LIB_PATH = os.environ.get("SDMI_LIB") or os.path.join(_HERE, "csrc", "libsdmi_hi
 SDMI_OK = 0
 DTYPE_BF16, DTYPE_F16, DTYPE_F32_PLANES, DTYPE_F16_TO_BF16, DTYPE_F32 = 0, 1, 2, 3, 4
 MX_NONE, MX_FP8, MX_FP4 = 0, 1, 2
+MX_KSTEP = 128            # K of block-scaled activations is held in whole steps of it
 RMSNORM_MAX_C = 16384
 MX_ALGOS = 8
 

@@ -401,8 +401,8 @@ def _auto_split_k(m, n_w, k, tile_n=_BN):
 _AUTO_SPLIT_K = _auto_split_k
 
 
-# Optional per-launch instrumentation (bench.py's roofline leg): when TRACE is a list, every sdmi_gemm
-# launch appends (kind, algorithmic_flops, start_event, end_event) recorded on the launch stream.
+# Optional per-launch instrumentation (bench.py's roofline leg): when TRACE is a list, every sdmi_gemm, norm, attention and
+# block-scaled call appends (kind, algorithmic work, start_event, end_event, split_k, shape) recorded on the launch stream.
 TRACE = None
 
 
@@ -915,15 +915,39 @@ def _mx_rows(t, name):
     return rows, k, ld
 
 
+def _mx_traced_as(what, args):
+    """(kind, work, shape) of a block-scaled call for TRACE, from the arguments of its C entry: bytes read and written of the
+    row-wise operators, FLOPs of the product."""
+    size = lambda dtype: 4 if dtype == hip.DTYPE_F32 else 2
+    held = lambda rows, k, fmt: rows * (-(-k // hip.MX_KSTEP)) * ((hip.MX_KSTEP if fmt == hip.MX_FP8 else hip.MX_KSTEP // 2) + 4)
+    if what == "sdmi_mx_quantize":
+        _, _, rows, k, dtype, _, _, fmt = args
+        return "mx_quantize", rows * k * size(dtype) + held(rows, k, fmt), (rows, k)
+    if what == "sdmi_mx_dequantize":
+        _, _, rows, k, fmt, _, _, dtype = args
+        return "mx_dequantize", rows * k * size(dtype) + held(rows, k, fmt), (rows, k)
+    if what == "sdmi_rmsnorm":
+        _, _, res, _, _, _, rows, c, dtype, _, _, out_dtype, _, fmt = args
+        out = held(rows, c, fmt) if fmt else rows * c * size(out_dtype)
+        return "rmsnorm", rows * c * size(dtype) * (1 if res is None else 3) + 4 * c + out, (rows, c)
+    if what == "sdmi_gated":
+        _, _, rows, c, dtype, _, _, out_dtype, _, fmt = args
+        return "gated", 2 * rows * c * size(dtype) + (held(rows, c, fmt) if fmt else rows * c * size(out_dtype)), (rows, c)
+    a = args[0]._obj
+    return "linear_mx", 2 * a.M * a.N * a.K, (a.M, a.N, a.K)
+
+
 def _mx_call(fn, what, device, *args):
     """fn(*args, stream) on `device` and its current stream.  Operators of a few microseconds: the raw handle is asked for
     where torch.cuda.current_stream() would make an object first (0.1 us for 2.8)."""
     index = device.index
-    if index == torch._C._cuda_getDevice():
-        st = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
-            st = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+            return _mx_call(fn, what, device, *args)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if TRACE is not None and what != "sdmi_mx_pack_linear":          # (packing is no part of a step)
+        return _traced(*_mx_traced_as(what, args), lambda: hip.check(fn(*args, stream), what))
+    st = fn(*args, stream)
     if st != hip.SDMI_OK:
         hip.check(st, what)
 

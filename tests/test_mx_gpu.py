@@ -666,3 +666,38 @@ def test_more_rows_than_a_launch_holds(dev, op):
         for (a, b), w in zip(windows, alone):
             assert torch.equal(y[a:b], w), (i, a)
         assert int(torch.count_nonzero(y)) == sum(int(torch.count_nonzero(w)) for w in alone), i
+
+
+# ----------------------------------------------------------------------------- in a traced step
+
+
+def test_the_operators_are_seen_by_the_trace(dev, monkeypatch):
+    """A traced step lists these calls with the others, each with its work, its sizes and the events around it; a refused call
+    leaves no entry, and the results are those of an untraced step."""
+    from stablediffusion_amd import hip
+    o = ops()
+    gamma, beta = torch.ones(256, device=dev), torch.zeros(256, device=dev)
+    x = data(40, 256, 1).to(dev)
+    pw = o.pack_linear_mx(torch.randn(512, 256, generator=torch.Generator().manual_seed(1)).to(dev))
+
+    def step():
+        y, s = o.rmsnorm(x, gamma, res=x, fmt="mxfp8")
+        h = o.linear_mx(y, pw)
+        a = o.gated(h, act="silu")
+        q = o.mx_quantize(a, "mxfp4")
+        return s, o.mx_dequantize(q), o.rmsnorm(x, gamma, out_dtype=torch.float32), o.linear_mx(x, pw), o.layernorm(x, gamma, beta)
+
+    want = step()
+    monkeypatch.setattr(o, "TRACE", [])
+    got = step()
+    with pytest.raises(hip.SdmiError):
+        o.linear_mx(x, pw, out_dtype=torch.int8)
+    o.pack_linear_mx(x)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    plain, codes8, codes4 = 40 * 256 * 2, 40 * (256 + 8), 40 * (128 + 8)
+    assert [(k, w, shape) for k, w, _, _, _, shape in o.TRACE] == [
+        ("rmsnorm", 3 * plain + 1024 + codes8, (40, 256)), ("linear_mx", 2 * 40 * 512 * 256, (40, 512, 256)), ("gated", 3 * plain, (40, 256)),
+        ("mx_quantize", plain + codes4, (40, 256)), ("mx_dequantize", codes4 + 2 * plain, (40, 256)),
+        ("rmsnorm", plain + 1024 + 2 * plain, (40, 256)), ("linear_mx", 2 * 40 * 512 * 256, (40, 512, 256)), ("layernorm", 2 * plain, (40, 256))]
+    assert all(e0.elapsed_time(e1) > 0 for _, _, e0, e1, _, _ in o.TRACE)
