@@ -701,3 +701,61 @@ def test_the_operators_are_seen_by_the_trace(dev, monkeypatch):
         ("mx_quantize", plain + codes4, (40, 256)), ("mx_dequantize", codes4 + 2 * plain, (40, 256)),
         ("rmsnorm", plain + 1024 + 2 * plain, (40, 256)), ("linear_mx", 2 * 40 * 512 * 256, (40, 512, 256)), ("layernorm", 2 * plain, (40, 256))]
     assert all(e0.elapsed_time(e1) > 0 for _, _, e0, e1, _, _ in o.TRACE)
+
+
+# ----------------------------------------------------------------------------- far offsets of the product
+
+
+@pytest.mark.parametrize("fmt,k", [("mxfp8", 4224), ("mxfp4", 8448)])
+def test_product_of_codes_past_32_bits(dev, monkeypatch, fmt, k):
+    """Codes past 2^32 bytes from the last k-steps on, in each kernel and from plain activations: the last rows bit for bit what
+    the same kernel makes of them alone (the tiled kernels add in one order, the direct ones in another), and those within the
+    product's bound of the 64-bit oracle.  The other rows are ones, all with the same result, so that an offset that wraps
+    reads other codes; a last k-step left out is over that bound in every row, in 80 % (mxfp8) and 63 % (mxfp4) of the elements."""
+    o = ops()
+    rows, n, tail_rows = 65535 * 16, 72, 200                   # (the most rows of the direct kernels of 16)
+    tail = data(tail_rows, k, 3, loud=False).to(dev)
+    w = torch.randn(n, k, generator=torch.Generator().manual_seed(1)) * k ** -0.5
+    pw = o.pack_linear_mx(w.to(dev))
+    x = torch.ones(rows, k, dtype=torch.bfloat16, device=dev)
+    x[-tail_rows:] = tail
+    q, alone, one = o.mx_quantize(x, fmt), o.mx_quantize(tail, fmt), o.mx_quantize(x[:1], fmt)
+    assert (k // 128 - 2) * rows * (128 if fmt == "mxfp8" else 64) < 2 ** 32 < q.codes.numel()
+    want, tol = product(O.values(tail.double().cpu(), fmt), O.values(w.double(), "mxfp4"), fmt, None, None)
+    for algo in range(1, 9):
+        monkeypatch.setattr(o, "FORCE_MX_ALGO", algo)
+        y, a = o.linear_mx(q, pw, out_dtype=torch.float32), o.linear_mx(alone, pw, out_dtype=torch.float32)
+        assert bool(((a.double().cpu() - want).abs() <= tol).all()), algo
+        assert torch.equal(y[-tail_rows:], a), algo
+        assert bool((y[:-tail_rows] == o.linear_mx(one, pw, out_dtype=torch.float32)).all()), algo
+        if algo in (1, 8):
+            assert torch.equal(o.linear_mx(x, pw, fmt=fmt, out_dtype=torch.float32), y), algo
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("algo", range(1, 9))
+def test_product_into_places_past_32_bits(dev, monkeypatch, algo, dtype):
+    """Outputs and residuals past 2^31 elements (2^32 bytes of bf16, 2^33 of fp32), one k-step, columns that end inside a quad: rows
+    at the start, across 2^31 elements and at the end are what the kernel makes of them alone, the others 0."""
+    o = ops()
+    monkeypatch.setattr(o, "FORCE_MX_ALGO", algo)
+    rows, n, k, t = (1 << 18) + 77, 8251, 100, TYPES[dtype]
+    border = (1 << 31) // n
+    windows = [(0, 60), (border - 70, border + 70), (rows - 300, rows)]
+    assert border + 70 < rows - 300 and rows * n > 1 << 31
+    g = torch.Generator().manual_seed(algo)
+    pw = o.pack_linear_mx((torch.randn(n, k, generator=g) * k ** -0.5).to(dev))
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device=dev)
+    wide = torch.zeros(rows, n + 5, dtype=t, device=dev)
+    res = wide[:, 3:3 + n]
+    parts = [(data(b - a, k, i + 1, loud=False).to(dev), torch.randn(b - a, n, generator=g).to(t).to(dev)) for i, (a, b) in enumerate(windows)]
+    for (a, b), (px, pr) in zip(windows, parts):
+        x[a:b], res[a:b] = px, pr
+    fmt = ["mxfp8", "mxfp4"][algo % 2]
+    y = o.linear_mx(o.mx_quantize(x, fmt), pw, res=res, out_dtype=t)
+    left = int(torch.count_nonzero(y))
+    for (a, b), (px, pr) in zip(windows, parts):
+        alone = o.linear_mx(o.mx_quantize(px, fmt), pw, res=pr, out_dtype=t)
+        assert torch.equal(y[a:b], alone), a
+        left -= int(torch.count_nonzero(alone))
+    assert left == 0
