@@ -130,9 +130,10 @@ __device__ __forceinline__ void mx_quad_store(const MxGemmDev& p, int64_t m, int
 // are neighbouring TOKENS: stored as they lie, a kilobyte of output is 64 addresses in 16 half lines.  So pairs of pieces (of
 // 16-bit types columns c and c + 32, of fp32 c and c + 4) go round the lanes until lane l holds piece l % 8 of a 128-byte line of
 // token l / 8, in the first of the two for tokens 0 ... 7 of the fragment and in the second for 8 ... 15; residuals take the same
-// way back.  (8192 x 10240 x 1280, 256 x 256 tiles, us: 4 bits 90 -> 86, with residual 121 -> 117; 4096 x 10240 x 1280 fp32
-// 86 -> 79.  Stores past the caches gain nothing, and whatever reads the output next has to fetch it from memory: 8192 x 10240 x
-// 5120 with the quantisation of its output 241 us, and 232 like this.)
+// way back.  (Before and after, with the bands of 4 and 8 tiles of that time: 8192 x 10240 x 1280, 256 x 256 tiles, 4 bits 90 and
+// 86 us, with residual 121 and 117; 4096 x 10240 x 1280 fp32 86 and 79.  Stores past the caches gained nothing, and whatever
+// reads the output next had to fetch it from memory: 8192 x 10240 x 5120 with the quantisation of its output 241 us, and 232
+// like this.)
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 __attribute__((aligned(2))) mx_u32x4_a2;
 __device__ __forceinline__ void mx_swap_rows(u32x4& a, u32x4& b, bool upper) {       // rows 0 - 7's b for rows 8 - 15's a; its own inverse
@@ -691,17 +692,17 @@ static bool mx_args_ok(const sdmi_mx_gemm_args* a) {
 // launch costs `fixed` us, a unit of K `first` for the first workgroup on each of the 256 CUs, and every further round of them
 // `round` and `more` a unit.  (Direct kernels: the unit is eight k-steps, one for each wave; tiled ones: one k-step.)  Least
 // squares over a sweep of 1 ... 8192 rows and twenty (N, K) from 320 x 320 to 20480 x 2560 and 5120 x 10240, of each kernel
-// where it takes at most 1.2 or 1.3 times as long as the fastest; the kernel picked is within 0.5 % of the fastest one on average and
-// 13 % at worst (1 x 640 x 640, 0.6 us).  Examples, us, 8-bit activations (direct kernels by their outputs a
-// workgroup, D, tiled ones T):
-//     32 x 10240 x 5120: D 32 x 64  9.4, D 48 x 64 10.4, D 16 x 64 12.4, D 16 x 32 12.7
-//     48 x  5120 x 5120: D 16 x 64  7.7, D 32 x 64  8.4, D 16 x 32  9.2, D 48 x 64 10.4
-//    128 x  5120 x 5120: D 48 x 64 10.8, D 32 x 64 14.1, T 64 x 128 15.4, T 128 x 128 21.0
-//    256 x  1280 x 1280: D 32 x 64  4.9, D 48 x 64  5.5, T 64 x 128  6.7, T 128 x 128  8.5
-//    512 x  5120 x 1280: T 128 x 128  9.4, T 64 x 128  9.5, D 48 x 64 15.8, T 256 x 256 16.9
-//   1024 x  5120 x 5120: T 64 x 128 30.7, T 128 x 256 30.9, T 128 x 128 32.5, T 256 x 256 47.7
-//   4096 x  5120 x 5120: T 128 x 128 84.9, T 64 x 128 96.9, T 256 x 256 102.4 (320 tiles: two rounds)
-//   8192 x  5120 x 5120: T 256 x 256 164, T 128 x 256 171, T 128 x 128 174
+// at the sizes where it is near the fastest; over the sweep the pick takes 1.005 (8-bit) and 1.003 (4-bit) times the fastest
+// one's time on average, 1.11 at worst (32 x 640 x 640, half a microsecond; profiles/mx_kernel_choice.txt has all of it).
+// Examples, us, 8-bit activations (direct kernels by their outputs a workgroup, D, tiled ones T):
+//     32 x 10240 x 5120: D 32 x 64  9.4, D 48 x 64 10.5, D 16 x 64 12.4, D 16 x 32 12.7
+//     48 x  5120 x 5120: D 16 x 64  7.7, D 32 x 64  8.5, D 16 x 32  9.3, D 48 x 64 10.4
+//    128 x  5120 x 5120: D 48 x 64 10.8, D 32 x 64 14.1, T 64 x 128 15.4, T 128 x 128 21.1
+//    256 x  1280 x 1280: D 32 x 64  4.9, D 48 x 64  5.5, T 64 x 128  6.6, T 128 x 128  8.5
+//    512 x  5120 x 1280: T 128 x 128  9.5, T 64 x 128  9.6, D 48 x 64 16.0, T 256 x 256 17.0
+//   1024 x  5120 x 5120: T 64 x 128 30.2, T 128 x 256 30.8, T 128 x 128 32.8, T 256 x 256 47.7
+//   4096 x  5120 x 5120: T 128 x 128 82.3, T 64 x 128 94.3, T 256 x 256 99.8 (320 tiles: two rounds)
+//   8192 x  5120 x 5120: T 256 x 256 158, T 128 x 256 158, T 128 x 128 164
 // Activations are read again by every column group and weights by every row tile, from L2, which is what the direct kernels'
 // shapes trade (96 x 5120 x 5120: 48 x 32 and 64 x 32 15.2 and 15.3 us, 32 x 64 8.9).
 // Parts of K in several workgroups of a tiled kernel and a second launch that joins them were measured too (two and four parts)
@@ -827,9 +828,11 @@ template <int FMT> static int mx_launch(const MxGemmDev& d, MxKind kind, MxFused
         case MX_D32x64: return direct_launch<FMT, 2, 4, 8, 1, -1>(d, st);
         case MX_D48x64: return direct_launch<FMT, 3, 4, 8, 1, -1>(d, st);
         // Rings no deeper than leaves room for three workgroups on a CU, whose starts and stores then run under each other's
-        // products (4096 x 10240 x 1280, 64 x 128: 8 bits 76.8 -> 69.5 us, 4 bits 62.0 -> 53.5; 128 x 128, 4 bits 48.9 -> 44.8); with
-        // 8-bit operands that is two stages of 128 x 128, which wait for their loads when they are alone on a CU
-        // (512 x 5120 x 5120, 160 tiles: 24.1 us with three stages, 29.8 with two; 4096 x 5120 x 5120, 1280 tiles: 95.7 and 90.8).
+        // products (with an earlier epilogue, 4096 x 10240 x 1280, 64 x 128: 8 bits 76.8 -> 69.5 us, 4 bits 62.0 -> 53.5; 128 x 128,
+        // 4 bits 48.9 -> 44.8).  With 8-bit operands that is two stages of 128 x 128, which wait for their loads when they are few
+        // on a CU.  Two and three stages, us: 160 tiles (512 x 5120 x 5120) 29.7 and 23.9, 480 (1536 x 5120 x 5120) 38.1 and 36.5,
+        // 520 (1664 x 5120 x 2560) 28.2 and 31.0, 1000 (3200 x 5120 x 5120) 70.7 and 68.1, 1280 (4096 x 5120 x 5120) 83.5 and 85.8, 2560
+        // (4096 x 10240 x 1280) 49.5 and 54.9.
         case MX_T64x128: return tiled_launch<FMT, 64, 2, 2, 3>(d, st);
         case MX_T128x128:
             if constexpr (FMT == SDMI_MX_FP8)
