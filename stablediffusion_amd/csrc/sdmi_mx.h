@@ -140,7 +140,7 @@ template <int FMT> __device__ __forceinline__ unsigned mx_quantise8(const float*
 // results show nothing of their errors (half a step is 2^-12 of a value at least); F32, the form for fp32 results, takes out the one error
 // that grows with |x|, the rounding of the exponential's argument.
 
-// 2^-(c m) for m in [0, 200]: c m as a rounded product and its remainder, c in two parts; exact but for exp2's own step.
+// 2^-(c m) for finite m >= 0: c m as a rounded product and its remainder, c in two parts; exact but for exp2's own step.
 __device__ __forceinline__ float mx_exp2_neg(float m, float c, float c_low) {
     const float t = m * c, low = fmaf(m, c_low, fmaf(m, c, -t));
     const float e = __builtin_amdgcn_exp2f(-t);
@@ -173,16 +173,31 @@ template <bool F32> __device__ __forceinline__ float mx_gelu(float x) {
 }
 
 // SiLU, x / (1 + exp(-x)).  The result is a normal fp32 number down to x = -91.6, exp(-x) only up to 88.7 and its reciprocal to
-// 87.3, so both are taken 2^-8 smaller.  The last scaling rounds the reciprocal to 17 bits out there: the form for fp32
-// results is written from exp(-|x|) = h^2 instead, whose root goes into the product twice (16384 x 5120 bf16, 4-bit result:
-// 88 us, and 91 in that form).
+// 87.3.  The form for fp32 results is therefore written from exp(-|x|) = h^2, whose root goes into the product twice; the
+// others take it for eight values at a time where one of them is below -87, and the plain form for all the rest (the plain form
+// alone 87.7 us at 16384 x 5120 bf16 with 4-bit results, the other one alone 91.6).
 template <bool F32> __device__ __forceinline__ float mx_silu(float x) {
     if constexpr (F32) {
         const float h = mx_exp2_neg(fminf(fabsf(x), 200.0f), MX_HALF_LOG2E, MX_HALF_LOG2E_LOW);       // exp(-|x| / 2)
         const float w = x < 0.0f ? h : 1.0f;
         return x * w * w * __builtin_amdgcn_rcpf(fmaf(h, h, 1.0f));
     } else {
-        const float e = __builtin_amdgcn_exp2f(fmaf(x, -2.0f * MX_HALF_LOG2E, -8.0f));
-        return x * (__builtin_amdgcn_rcpf(e + 0x1p-8f) * 0x1p-8f);
+        return silu_f(x);
     }
+}
+
+// f[j] *= gate(g[j]), OP 1 GELU, 2 SiLU
+template <int OP, bool F32> __device__ __forceinline__ void mx_gate8(float* f, const float* g) {
+    if constexpr (OP == 2 && !F32) {
+        unsigned most = 0u;                       // of the bits: -87 and further down, and negative NaN
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(g[j]));
+        if (most > __builtin_bit_cast(unsigned, -87.0f)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] *= mx_silu<true>(g[j]);
+            return;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] *= OP == 1 ? mx_gelu<F32>(g[j]) : mx_silu<F32>(g[j]);
 }

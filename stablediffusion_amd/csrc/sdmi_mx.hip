@@ -46,13 +46,7 @@ __global__ __launch_bounds__(256) void sdmi_mx_elem_kernel(MxElemArgs p) {
         if (step >= nsteps) break;                               // (uniform)
         const int64_t k0 = step * MX_KSTEP + sub * 8;
         const int n = (int)max((int64_t)0, min((int64_t)8, p.K - k0));
-        if constexpr (OP == 1) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[s][j] *= mx_gelu<FMT < 0 && TO == 2>(g[s][j]);
-        } else if constexpr (OP == 2) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[s][j] *= mx_silu<FMT < 0 && TO == 2>(g[s][j]);
-        }
+        if constexpr (OP != 0) mx_gate8<OP, FMT < 0 && TO == 2>(f[s], g[s]);
         if constexpr (FMT < 0) {
             if (row < p.rows && n > 0)
                 mx_store8<TO>(reinterpret_cast<typename MxElem<TO>::type*>(p.out) + row * p.ld_out + k0, n, f[s]);

@@ -566,10 +566,9 @@ def test_offsets_past_32_bits(dev, fmt):
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_silu_where_its_exponential_leaves_fp32(dev, dtype, fmt):
     """x / (1 + exp(-x)) is a normal fp32 number down to x = -91.6, exp(x) only down to -87.3 and 1 / exp(-x) down to -88.7.
-    fp32 results: the exponent |x| / (2 ln 2) is rounded, times a rounded constant, in a root and counts twice: 2 |x| 2^-24
-    relative, 183 2^-24 at 91.5 and 220 at 110.  Others: |x| 2^-24 and 20 for the constant, and a reciprocal of 2^-132 on the
-    grid of 2^-149, 71.  Both under GATE_REL = 256 2^-24 with a dozen roundings beside it.  Below the normal numbers the relative
-    error stays (1.2e-38 2^-16 = 130 steps of 2^-149), and two products are rounded to half a step each."""
+    The exponent |x| / (2 ln 2) rounded, times a rounded constant, in a root that counts twice would be 2 |x| 2^-24 relative, 183
+    2^-24 at 91.5 and 220 at 110: under GATE_REL = 256 2^-24 with a dozen roundings beside it.  Below the normal numbers the
+    relative error stays (1.2e-38 2^-16 = 130 steps of 2^-149), and two products are rounded to half a step each."""
     b = torch.linspace(-91.5, -60.0, 2048).to(TYPES[dtype])
     b = b[b >= -91.5]
     b = b[len(b) % 32:]                                        # (blocks of 32, in order: their values are alike)
